@@ -82,6 +82,28 @@ int fnx_hc_rms_norm(void* x, void* w, void* out, int batch, int H, int HC, float
 /* fnx_inject for any H % 8 == 0 and HC <= 64. */
 int fnx_inject_ex(void* h, void* y, void* g, void* out, int batch, int H, int HC, void* stream);
 
+/* The residual step between two blocks with the norms on both sides of it (inject,
+ * fnx/engine.py:859-877, then the rms_norm that opens the next gated_residual,
+ * fnx/engine.py:156-190, 818-857), with an optional norm of the block's output before the gate:
+ *   z = values, or values / rms(values) * (1 + w_post) with w_post bf16 [H];
+ *   state[t, b*H + c] = hyper[t, b*H + c] + scale * gate[t, b] * z[t, c];
+ *   normed[t, b*H + c] = state / rms(state[t, branch b]) * (1 + w_next[b*H + c]).
+ * hyper, state, normed bf16 [batch, HC*H], gate bf16 [batch, HC] (NULL: 1), values bf16 [batch, H],
+ * w_next bf16 [HC*H] (NULL with normed NULL: no second norm); rms(v) = sqrt(mean(v^2) + eps).
+ * fp32 inside, each output rounded once (normed from the unrounded state).  state may be hyper.
+ * H % 8 == 0, H <= 16384, HC <= 4, (HC + 2) * H <= 56000; all 16-byte aligned but gate. */
+int fnx_inject_norm(const void* hyper, const void* gate, const void* values, const void* w_post, const void* w_next,
+                    void* state, void* normed, int batch, int H, int HC, float scale, float eps, void* stream);
+/* Its gradients, from its stored state and its inputs: d_state, d_normed bf16 [batch, HC*H] (one of
+ * them may be NULL: zero) -> d_hyper [batch, HC*H], d_values [batch, H], and where not NULL d_gate
+ * [batch, HC], d_w_post [H], d_w_next [HC*H].  Sums over tokens in fp32 in a fixed order
+ * (deterministic).  ws: 16-byte aligned, fnx_inject_norm_backward_workspace(batch, H, HC) bytes. */
+size_t fnx_inject_norm_backward_workspace(int batch, int H, int HC);
+int fnx_inject_norm_backward(const void* d_state, const void* d_normed, const void* state, const void* gate,
+                             const void* values, const void* w_post, const void* w_next, void* d_hyper, void* d_gate,
+                             void* d_values, void* d_w_post, void* d_w_next, int batch, int H, int HC, float scale,
+                             float eps, void* ws, size_t ws_bytes, void* stream);
+
 /* fnx_gather_pair with any slot count; ids outside [0,E) copy zeros and set device error 2
  * (E <= 0 disables the check). */
 int fnx_gather_pair_ex(void* w, void* s, void* ids, void* ow, void* os, int E, int K, int G, int N, int nslots,

@@ -18,6 +18,7 @@
 #include "kernels_gemm_pair.cuh"
 #include "kernels_gemm_bf16.cuh"
 #include "kernels_hc.cuh"
+#include "kernels_inject_norm.cuh"
 #include "kernels_route.cuh"
 #include "kernels_w4gemv.cuh"
 #include "kernels_w8gemv.cuh"
@@ -382,6 +383,102 @@ FNX_API int fnx_moe_combine_inject(void* yd, void* wf, void* inverse, void* sh, 
         (const bf16*)yd, (const float*)wf, (const int64_t*)inverse, (const bf16*)sh, (const bf16*)gate, gate_ld,
         (bf16*)out, T, k, H, (const bf16*)hyper, (const bf16*)inj, (bf16*)out_hyper, HC);
     return launch_rc();
+}
+
+// ------------------------------------------------------------------ gated residual with its norms
+namespace {
+// the backward's column sums and dz of one token fill at most 224,000 bytes of shared memory
+constexpr int IN_MAX_H = 16384, IN_MAX_HC = 4, IN_MAX_SUMS = 56000;
+
+bool inject_norm_shape(int batch, int H, int HC) {
+    return batch >= 0 && H >= 8 && H % 8 == 0 && H <= IN_MAX_H && HC >= 1 && HC <= IN_MAX_HC &&
+           (long long)(HC + 2) * H <= IN_MAX_SUMS;
+}
+
+template <int NV, int BR>
+int inject_norm_launch_t(const InjectNormParams& p, int batch, cudaStream_t st) {
+    const int threads = ((p.H / 8 + NV - 1) / NV + 31) / 32 * 32;
+    inject_norm_kernel<NV, BR><<<dim3((unsigned)batch, (unsigned)((p.HC + BR - 1) / BR)), threads, 0, st>>>(p);
+    return launch_rc();
+}
+
+template <int BR>
+int inject_norm_launch(const InjectNormParams& p, int batch, cudaStream_t st) {
+    if (p.H <= 4096) return inject_norm_launch_t<1, BR>(p, batch, st);
+    if (p.H <= 8192) return inject_norm_launch_t<2, BR>(p, batch, st);
+    return inject_norm_launch_t<4, BR>(p, batch, st);
+}
+
+size_t inject_norm_bwd_smem(int H, int HC) { return (size_t)(HC + 2) * H * sizeof(float); }
+int inject_norm_bwd_blocks(int batch, int H, int HC) {
+    const int per_sm = inject_norm_bwd_smem(H, HC) <= 100 * 1024 ? 2 : 1;
+    const int g = per_sm * num_sms();
+    return batch < g ? batch : g;
+}
+}  // namespace
+
+FNX_API int fnx_inject_norm(const void* hyper, const void* gate, const void* values, const void* w_post,
+                            const void* w_next, void* state, void* normed, int batch, int H, int HC, float scale,
+                            float eps, void* stream) {
+    if (!inject_norm_shape(batch, H, HC)) return FNX_ESHAPE;
+    if (batch == 0) return FNX_OK;                    // an empty tensor has no address
+    if (!hyper || !values || !state || (!w_next != !normed)) return FNX_EARG;
+    if (!aligned16(hyper) || !aligned16(values) || !aligned16(state) || (w_post && !aligned16(w_post)) ||
+        (w_next && (!aligned16(w_next) || !aligned16(normed))))
+        return FNX_EALIGN;
+    const InjectNormParams p{(const bf16*)hyper, (const bf16*)gate, (const bf16*)values, (const bf16*)w_post,
+                             (const bf16*)w_next, (bf16*)state, (bf16*)normed, H, HC, scale, eps};
+    cudaStream_t st = (cudaStream_t)stream;
+    if (HC == 1 || batch < num_sms()) return inject_norm_launch<1>(p, batch, st);
+    if (HC == 2) return inject_norm_launch<2>(p, batch, st);
+    return inject_norm_launch<4>(p, batch, st);
+}
+
+FNX_API size_t fnx_inject_norm_backward_workspace(int batch, int H, int HC) {
+    if (!inject_norm_shape(batch, H, HC)) return 0;
+    return (size_t)inject_norm_bwd_blocks(batch, H, HC) * (HC + 1) * H * sizeof(float);
+}
+
+FNX_API int fnx_inject_norm_backward(const void* d_state, const void* d_normed, const void* state, const void* gate,
+                                     const void* values, const void* w_post, const void* w_next, void* d_hyper,
+                                     void* d_gate, void* d_values, void* d_w_post, void* d_w_next, int batch, int H,
+                                     int HC, float scale, float eps, void* ws, size_t ws_bytes, void* stream) {
+    if (!inject_norm_shape(batch, H, HC)) return FNX_ESHAPE;
+    if (batch && ((!d_state && !d_normed) || !state || !values || !d_hyper || !d_values || (d_gate && !gate)))
+        return FNX_EARG;                              // an empty tensor has no address
+    if ((d_normed && !w_next) || (d_w_post && !w_post) || (d_w_next && !w_next)) return FNX_EARG;
+    for (const void* q : {d_state, d_normed, state, values, w_post, w_next, (const void*)d_hyper,
+                          (const void*)d_values, (const void*)ws})
+        if (!aligned16(q)) return FNX_EALIGN;
+    const size_t need = fnx_inject_norm_backward_workspace(batch, H, HC);
+    if (ws_bytes < need || (need && !ws)) return FNX_EWORKSPACE;
+    cudaStream_t st = (cudaStream_t)stream;
+    const int blocks = inject_norm_bwd_blocks(batch, H, HC);
+    if (batch) {
+        static bool configured[FNX_MAX_DEVICES] = {};
+        const int dev = current_device();
+        if (!configured[dev]) {
+            if (cudaFuncSetAttribute(inject_norm_bwd_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     IN_MAX_SUMS * (int)sizeof(float)) != cudaSuccess)
+                return FNX_ELAUNCH;
+            configured[dev] = true;
+        }
+        const InjectNormBwdParams p{(const bf16*)d_state, (const bf16*)d_normed, (const bf16*)state, (const bf16*)gate,
+                                    (const bf16*)values, (const bf16*)w_post, (const bf16*)w_next, (bf16*)d_hyper,
+                                    (bf16*)d_gate, (bf16*)d_values, (float*)ws, batch, H, HC, scale, eps};
+        int threads = (H / 8 + 31) / 32 * 32;
+        if (threads > 512) threads = 512;
+        inject_norm_bwd_kernel<<<blocks, threads, inject_norm_bwd_smem(H, HC), st>>>(p);
+        const int rc = launch_rc();
+        if (rc) return rc;
+    }
+    if (d_w_next || d_w_post) {
+        const int n = (HC + 1) * H;
+        column_sum_kernel<<<(n + 31) / 32, 256, 0, st>>>((const float*)ws, (bf16*)d_w_next, (bf16*)d_w_post, blocks,
+                                                         HC * H, n);
+        return launch_rc();
+    }
+    return FNX_OK;
 }
 
 // ------------------------------------------------------------------ hyper-connection mix

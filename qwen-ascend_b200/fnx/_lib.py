@@ -7,6 +7,7 @@ no fallback: if the library or a CUDA device is missing, the call raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from pathlib import Path
 
@@ -16,6 +17,7 @@ P = ctypes.c_void_p
 I = ctypes.c_int
 LL = ctypes.c_longlong
 SZ = ctypes.c_size_t
+F = ctypes.c_float
 
 # name -> (argtypes, restype)
 SIGNATURES = {
@@ -37,6 +39,9 @@ SIGNATURES = {
     "fnx_hc_sigmoid_reduce": ([P] * 3 + [I, P], I),
     "fnx_hc_sigmoid_reduce_ex": ([P] * 3 + [I] * 3 + [P], I),
     "fnx_inject_ex": ([P] * 4 + [I, I, I, P], I),
+    "fnx_inject_norm": ([P] * 7 + [I, I, I, F, F, P], I),
+    "fnx_inject_norm_backward_workspace": ([I] * 3, SZ),
+    "fnx_inject_norm_backward": ([P] * 12 + [I, I, I, F, F, P, SZ, P], I),
     "fnx_router_topk": ([P, LL, P, P, P, P, I, I, I, P], I),
     "fnx_moe_permute_workspace": ([I, I], SZ),
     "fnx_moe_permute": ([P] * 5 + [I, I, P, SZ, P], I),
@@ -110,6 +115,19 @@ def lib():
 
 def stream(device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def on_device(fn):
+    """Runs ``fn(first tensor, ...)`` with that tensor's device current, where it is not already (the
+    library launches on the current device)."""
+    @functools.wraps(fn)
+    def call(self_or_tensor, *args, **kw):
+        t = self_or_tensor if isinstance(self_or_tensor, torch.Tensor) else args[0] if args else None
+        if isinstance(t, torch.Tensor) and t.is_cuda and t.device.index != torch.cuda.current_device():
+            with torch.cuda.device(t.device):
+                return fn(self_or_tensor, *args, **kw)
+        return fn(self_or_tensor, *args, **kw)
+    return call
 
 
 def ptr(t) -> int | None:

@@ -100,7 +100,7 @@ def mm_nt(x, w):
     return out
 
 
-def gated_residual(h, hc_norm_w, w_down, w_up, w_inj=None, n_inj=0, hc=4, eps=1e-6, moe=None):
+def gated_residual(h, hc_norm_w, w_down, w_up, w_inj=None, n_inj=0, hc=4, eps=1e-6, moe=None, normed=None):
     """The hyper-connection mix that produces a layer's MoE input (``fnx/engine.py:818-857``):
     ``h`` bf16 ``[b, 1, hc*H]`` -> ``(mixed [b, 1, H], inj [b, 1, hc])``.  ``w_down`` bf16
     ``[r (+ hc), hc*H]`` (with ``n_inj == hc`` its last rows are the inject weights, as the
@@ -112,18 +112,24 @@ def gated_residual(h, hc_norm_w, w_down, w_up, w_inj=None, n_inj=0, hc=4, eps=1e
     (``MoELayer.mix_and_route``) and its decode must be called next with ``logits_ready=True``.
     Same bits either way; on B200 the fused pair is the slower one (25.6 against 23.0 us per layer
     at b = 1), because the decode kernel already overlaps its own router GEMV with the
-    expert-weight stream."""
+    expert-weight stream.  ``normed``: the rms norm of ``h`` with ``hc_norm_w`` where the residual
+    step before this one has made it already (``native_inject.inject_norm``); no norm runs then."""
     from . import post_ops
     b, HCH = h.shape[0], h.shape[-1]
     H = HCH // hc
     if moe is not None and (b > DECODE_MAX_TOKENS or moe.E > DECODE_MAX_EXPERTS or moe.H != H):
         raise ValueError(f"gated_residual: the fused router needs b <= {DECODE_MAX_TOKENS}, E <= "
                          f"{DECODE_MAX_EXPERTS} and the layer's H = {H} (got b={b}, E={moe.E}, H={moe.H})")
-    h2 = h.reshape(b, HCH).contiguous()
-    hn = torch.empty_like(h2)
-    rc = _lib.lib().fnx_hc_rms_norm(h2.data_ptr(), hc_norm_w.contiguous().data_ptr(), hn.data_ptr(), b, H, hc, eps,
-                                    _lib.stream(h.device))
-    _lib.check(rc, "hyper-connection rms_norm")
+    if normed is None:
+        h2 = h.reshape(b, HCH).contiguous()
+        hn = torch.empty_like(h2)
+        rc = _lib.lib().fnx_hc_rms_norm(h2.data_ptr(), hc_norm_w.contiguous().data_ptr(), hn.data_ptr(), b, H, hc, eps,
+                                        _lib.stream(h.device))
+        _lib.check(rc, "hyper-connection rms_norm")
+    elif normed.shape != h.shape or normed.dtype != BF16 or normed.device != h.device:
+        raise ValueError("gated_residual: normed must be bf16, shaped and placed like h")
+    else:
+        hn = normed.reshape(b, HCH).contiguous()
     if not n_inj:
         if w_inj is None:
             raise ValueError("gated_residual: pass w_inj, or w_down with the inject rows and n_inj = hc")
