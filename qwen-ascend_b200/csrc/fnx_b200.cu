@@ -20,6 +20,7 @@
 #include "kernels_hc.cuh"
 #include "kernels_inject_norm.cuh"
 #include "kernels_route.cuh"
+#include "kernels_w4dense.cuh"
 #include "kernels_w4gemv.cuh"
 #include "kernels_w8gemv.cuh"
 
@@ -1132,6 +1133,53 @@ FNX_API int fnx_bf16_gemm_nt(const void* x, long long ld_x, const void* w, void*
     }
     if (N % 160 == 0) return gemm_bf16_tma_launch_t<160>(x, ld_x, w, y, ld_y, M, K, N, st);
     return gemm_bf16_tma_launch_t<128>(x, ld_x, w, y, ld_y, M, K, N, st);
+}
+
+// ======================================================================== dense W4
+namespace {
+template <int WPL, int NT>
+int w4_dense_launch_t(const W4DenseParams& p, int CL, cudaStream_t st) {
+    static bool configured[FNX_MAX_DEVICES] = {};
+    const int dev = current_device();
+    if (!configured[dev]) {
+        if (cudaFuncSetAttribute(w4_dense_kernel<WPL, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 (int)w4_dense_smem<WPL, NT>(8 * NT)) != cudaSuccess)
+            return FNX_ELAUNCH;
+        configured[dev] = true;
+    }
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1;
+    attr[0].val.clusterDim.y = (unsigned)CL;
+    attr[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((p.N + W4D_FEATS - 1) / W4D_FEATS), (unsigned)CL, (unsigned)((p.M + 8 * NT - 1) / (8 * NT)));
+    cfg.blockDim = dim3(W4D_THREADS, 1, 1);
+    cfg.dynamicSmemBytes = w4_dense_smem<WPL, NT>(p.M);
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, w4_dense_kernel<WPL, NT>, p) != cudaSuccess) return FNX_ELAUNCH;
+    return launch_rc();
+}
+}  // namespace
+
+FNX_API int fnx_w4a16_gemv(const void* x, long long ld_x, const void* w4, const void* scales, void* y, int M, int K,
+                           int N, int gs, void* stream) {
+    if (M < 0 || K < 8 || N < 8 || gs < 16 || gs % 16 || ld_x < K) return FNX_EARG;
+    if (K % 8 || N % 8 || M > 16 * 65535) return FNX_ESHAPE;
+    if (M == 0) return FNX_OK;
+    if (!x || !w4 || !scales || !y) return FNX_EARG;
+    if (!aligned16(x) || !aligned16(w4) || !aligned16(scales) || !aligned16(y) || ld_x % 4) return FNX_EALIGN;
+    const W4DenseParams p{(const bf16*)x, (const uint32_t*)w4, (const bf16*)scales, (bf16*)y, ld_x, M, K, N, gs};
+    const int NT = M <= 8 ? 1 : 2;
+    const long long tiles = (long long)((N + W4D_FEATS - 1) / W4D_FEATS) * ((M + 8 * NT - 1) / (8 * NT));
+    int CL = 1;
+    while (CL < 8 && tiles * CL < 2 * num_sms() && K / (16 * CL) >= 16) CL *= 2;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (NT == 2) return w4_dense_launch_t<1, 2>(p, CL, st);
+    if (N % 16 == 0) return w4_dense_launch_t<2, 1>(p, CL, st);
+    return w4_dense_launch_t<1, 1>(p, CL, st);
 }
 
 // ======================================================================== load-time repack

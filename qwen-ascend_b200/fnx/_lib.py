@@ -79,6 +79,7 @@ SIGNATURES = {
     "fnx_w8a16_gemm": ([P] * 4 + [I] * 4 + [P], I),
     "fnx_w8a16_gemm_workspace": ([I] * 4, SZ),
     "fnx_w8a16_gemm_ws": ([P] * 4 + [I] * 4 + [P, SZ, P], I),
+    "fnx_w4a16_gemv": ([P, LL, P, P, P] + [I] * 4 + [P], I),
     "fnx_bf16_gemm_nt": ([P, LL, P, P, LL, I, I, I, P], I),
     "fnx_moe_decode_workspace": ([I] * 5, SZ),
     "fnx_moe_decode_w4": ([P] * 10 + [I] * 5 + [P, SZ, P], I),
@@ -115,6 +116,12 @@ def lib():
 
 def stream(device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def raw_stream(device) -> int:
+    """``stream(device)`` for a device with an index, without building a stream object (a decode
+    step's host time is made of such calls)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def on_device(fn):

@@ -8,6 +8,8 @@ Mirrors the reference's MoE/quant section of ``fnx/engine.py``:
   the LQP ``v2o`` artifact; ``matmul`` runs the same grouped GEMM per selected expert.
 * ``DenseW8`` (reference ``fnx/engine.py:297-384``): int8 ``[K, N]`` + bf16 ``[G, N]``
   scales, N-concatenation by ``merge``; calls run the W8A16 kernels.
+* ``DenseW4``: dense int4pack weights + bf16 group scales for the decode batch, beside
+  ``DenseW8``; calls run the W4A16 GEMV.
 * ``MoELayer`` (reference ``FnLayer._moe``, ``fnx/engine.py:1782-1930``): shared expert,
   router top-k, expert-major permutation, grouped gate/up + SwiGLU, grouped down,
   slot-order combine and sigmoid-gated shared merge.  ``T <= 16`` tokens take the fused
@@ -379,6 +381,61 @@ class DenseW8:
         o.gs, o.K, o.N = gs, parts[0].K, o.w8t.shape[1]
         o.chunks = None
         return o
+
+
+class DenseW4:
+    """Dense int4 weights with per-group bf16 scales, the 4-bit form of ``DenseW8`` for the decode
+    batch: ``w4`` int32 ``[K, N/8]`` int4pack words (``tools/repack_w4a16.py``'s layout without the
+    expert axis, read unchanged) and ``sc`` bf16 ``[ceil(K/gs), N]``; a call gives
+    ``x [.., K] @ (q * s) -> bf16 [.., N]`` on the weight-streaming GEMV, accumulated in fp32 with the
+    scale applied to each group's exact sum (no weight is rounded, unlike the expert GEMM's
+    ``bf16(q * s)``).  The weights are read once for up to 16 rows; more rows are right but read
+    them again every 16.  K and N are multiples of 8, ``gs`` of 16."""
+
+    def __init__(self, w4, sc, gs):
+        if w4.dim() != 2 or w4.dtype != torch.int32 or sc.dim() != 2 or sc.dtype != BF16 or sc.device != w4.device:
+            raise ValueError("DenseW4: int32 words [K, N/8] and bf16 scales [G, N] on one device expected")
+        self.K, self.N, self.gs = w4.shape[0], w4.shape[1] * 8, gs
+        if self.K < 8 or self.K % 8 or self.N < 8 or gs < 16 or gs % 16 or tuple(sc.shape) != (-(-self.K // gs), self.N):
+            raise ValueError(f"DenseW4: K={self.K} must be a multiple of 8, gs={gs} of 16, and scales "
+                             f"[{-(-self.K // max(gs, 1))}, {self.N}], not {tuple(sc.shape)}")
+        _lib.require_cuda(w4)
+        self.w4, self.sc = w4.contiguous(), sc.contiguous()
+        if (self.w4.data_ptr() | self.sc.data_ptr()) % 16:
+            raise ValueError("DenseW4: weights and scales must be 16-byte aligned")
+        self._fn = _lib.lib().fnx_w4a16_gemv
+
+    def __call__(self, x):
+        if x.shape[-1] != self.K or x.device != self.w4.device:
+            raise ValueError(f"DenseW4: rows of {self.K} on {self.w4.device} expected, got {tuple(x.shape)} on {x.device}")
+        return self._run(x)
+
+    @_lib.on_device
+    def _run(self, x):
+        x2 = x if x.dtype == BF16 else x.to(BF16)
+        if x2.dim() != 2 or x2.stride(1) != 1 or x2.stride(0) % 4 or x2.stride(0) < self.K or x2.data_ptr() % 16:
+            x2 = x2.reshape(-1, self.K).contiguous()
+            if x2.data_ptr() % 16:
+                x2 = x2.clone()
+        M = x2.shape[0]
+        y = torch.empty(M, self.N, dtype=BF16, device=x2.device)
+        rc = self._fn(x2.data_ptr(), x2.stride(0) if M > 1 else self.K, self.w4.data_ptr(), self.sc.data_ptr(),
+                      y.data_ptr(), M, self.K, self.N, self.gs, _lib.raw_stream(x2.device))
+        _lib.check(rc, "W4A16 GEMV")
+        return y if x.dim() == 2 else y.view(*x.shape[:-1], self.N)
+
+    def deq_w(self):
+        """fp32 ``[N, K]``: the weights a call multiplies with."""
+        t = torch.arange(0, 32, 4, device=self.w4.device, dtype=torch.int32)
+        q = ((((self.w4[:, :, None] >> t) & 15) ^ 8) - 8).view(self.K, self.N).float()
+        return (q * self.sc.float().repeat_interleave(self.gs, dim=0)[:self.K]).t().contiguous()
+
+    @staticmethod
+    def merge(parts):
+        """N-concatenation, as ``DenseW8.merge``."""
+        if not parts or any(p.gs != parts[0].gs or p.K != parts[0].K for p in parts):
+            raise ValueError("DenseW4.merge: group size / K differ, cannot merge")
+        return DenseW4(torch.cat([p.w4 for p in parts], dim=1), torch.cat([p.sc for p in parts], dim=1), parts[0].gs)
 
 
 class MoELayer:
