@@ -305,6 +305,24 @@ int fnx_w8a16_gemm_ws(const void* x, const void* w8t, const void* sc, void* y, i
 int fnx_w4a16_gemv(const void* x, long long ld_x, const void* w4, const void* scales, void* y, int M, int K, int N,
                    int gs, void* stream);
 
+/* The bf16 gated feed-forward block (the always-on expert of fnx/engine.py:1786-1790 in the form the
+ * reference deploys it: one concatenated gate/up projection, silu(gate) * up, down):
+ *   h bf16 [M, I] = silu(x w_gu[:I]^T) * (x w_gu[I:]^T),  y bf16 [M, O] = h w_down^T
+ * x bf16 [M, ld_x], w_gu bf16 [2I, H] (gate rows, then up rows), w_down bf16 [O, I]; w_down and y
+ * may both be NULL (h alone).  Both projections, the activation and the product are one kernel with
+ * fp32 accumulators; h is rounded once (it is the next product's operand) and y once.  saved: NULL, or
+ * fnx_gated_ffn_saved_bytes(M, I) bytes that receive gate and up in fp32 for the backward (opaque).
+ * H, I, O, ld_x % 8 == 0; all pointers 16-byte aligned. */
+size_t fnx_gated_ffn_saved_bytes(int M, int I);
+int fnx_gated_ffn(const void* x, long long ld_x, const void* w_gu, const void* w_down, void* h, void* saved, void* y,
+                  int M, int H, int I, int O, void* stream);
+/* Its gradients from dy bf16 [M, ld_dy]: dx bf16 [M, H], dw_gu bf16 [2I, H], dw_down bf16 [O, I] (each
+ * may be NULL), with dgu bf16 [M, 2I] as scratch: the gradients of gate and up, whose activation
+ * derivative runs in the epilogue of dy w_down on its fp32 accumulators.  Deterministic. */
+int fnx_gated_ffn_backward(const void* dy, long long ld_dy, const void* x, long long ld_x, const void* w_gu,
+                           const void* w_down, const void* h, const void* saved, void* dgu, void* dx, void* dw_gu,
+                           void* dw_down, int M, int H, int I, int O, void* stream);
+
 /* bf16 GEMM y [M, N] = x [M, K] . w [N, K]^T with fp32 accumulation (the router / concatenated
  * shared GEMM, fnx/engine.py:1787; the hyper-connection mix's GEMMs, fnx/engine.py:818-857):
  * both operands by TMA into a tcgen05 pipeline.  K % 64 == 0, ld_x % 8 == 0, x and w 16-byte

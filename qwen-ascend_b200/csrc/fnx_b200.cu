@@ -14,6 +14,7 @@
 #include "kernels_decode.cuh"
 #include "kernels_decode2.cuh"
 #include "kernels_ep.cuh"
+#include "kernels_ffn.cuh"
 #include "kernels_gemm.cuh"
 #include "kernels_gemm_pair.cuh"
 #include "kernels_gemm_bf16.cuh"
@@ -1133,6 +1134,135 @@ FNX_API int fnx_bf16_gemm_nt(const void* x, long long ld_x, const void* w, void*
     }
     if (N % 160 == 0) return gemm_bf16_tma_launch_t<160>(x, ld_x, w, y, ld_y, M, K, N, st);
     return gemm_bf16_tma_launch_t<128>(x, ld_x, w, y, ld_y, M, K, N, st);
+}
+
+// ======================================================================== gated feed-forward block
+namespace {
+// A bf16 matrix as an operand or output of ffn_gemm_kernel: `cols` contiguous elements per row, rows
+// `ld` elements apart.  Encoded per call (no cache: half a microsecond of host time).
+int ffn_map(CUtensorMap* out, const void* ptr, long long cols, long long rows, long long ld, unsigned b0, unsigned b1) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return FNX_EDRIVER;
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
+    const cuuint32_t box[2] = {b0, b1};
+    const cuuint32_t estr[2] = {1, 1};
+    return fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? FNX_OK : FNX_EALIGN;
+}
+
+template <int AMN, int BMN, int EPI>
+int ffn_launch(const FfnParams& p, cudaStream_t st) {
+    const size_t smem = ffn_gemm_smem();
+    static int clusters_of[FNX_MAX_DEVICES] = {};
+    int& clusters = clusters_of[current_device()];
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.blockDim = dim3(FF_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (!clusters) {
+        if (cudaFuncSetAttribute(ffn_gemm_kernel<AMN, BMN, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 (int)smem) != cudaSuccess)
+            return FNX_ELAUNCH;
+        clusters = num_sms() / 2;
+    }
+    const int cols = EPI == FF_GATED ? 128 : 256;
+    const long long tiles = (long long)((p.M + FF_BM - 1) / FF_BM) * ((p.N + cols - 1) / cols);
+    if (tiles > 0x7fffffffLL) return FNX_ESHAPE;
+    cfg.gridDim = dim3((unsigned)(2 * (tiles < clusters ? tiles : clusters)));
+    cfg.stream = st;
+    if (cudaLaunchKernelEx(&cfg, ffn_gemm_kernel<AMN, BMN, EPI>, p) != cudaSuccess) return FNX_ELAUNCH;
+    return launch_rc();
+}
+
+// C [M, N] = A B^T; a, b: the stored matrices, K-major [M, K] / [N, K] or (amn, bmn) MN-major [K, M] / [K, N]
+template <int AMN, int BMN>
+int ffn_gemm(const void* a, long long lda, const void* b, long long ldb, void* c, long long ldc, int M, int N, int K,
+             cudaStream_t st) {
+    FfnParams p;
+    memset(&p, 0, sizeof p);
+    int rc = AMN ? ffn_map(&p.ta, a, M, K, lda, 64, 64) : ffn_map(&p.ta, a, K, M, lda, 64, 128);
+    if (!rc) rc = BMN ? ffn_map(&p.tb, b, N, K, ldb, 64, 64) : ffn_map(&p.tb, b, K, N, ldb, 64, 128);
+    if (!rc) rc = ffn_map(&p.tc, c, N, M, ldc, 64, 32);
+    if (rc) return rc;
+    p.M = M; p.N = N; p.K = K;
+    return ffn_launch<AMN, BMN, FF_PLAIN>(p, st);
+}
+
+int ffn_check(int M, int H, int I, int O) {
+    if (M < 0 || H < 8 || I < 8 || O < 8) return FNX_EARG;
+    if (H % 8 || I % 8 || O % 8 || I > (1 << 24) || H > (1 << 24) || O > (1 << 24) || M > (1 << 28)) return FNX_ESHAPE;
+    return FNX_OK;
+}
+}  // namespace
+
+FNX_API size_t fnx_gated_ffn_saved_bytes(int M, int I) {
+    if (M < 1 || I < 8 || I % 8) return 0;
+    return (size_t)((M + 127) / 128 * 128) * 2 * I * sizeof(float);
+}
+
+FNX_API int fnx_gated_ffn(const void* x, long long ld_x, const void* w_gu, const void* w_down, void* h, void* saved,
+                          void* y, int M, int H, int I, int O, void* stream) {
+    int rc = ffn_check(M, H, I, O);
+    if (rc) return rc;
+    if (M == 0) return FNX_OK;                        // an empty tensor has no address
+    if (!x || !w_gu || !h || (!w_down != !y) || ld_x < H) return FNX_EARG;
+    for (const void* q : {x, w_gu, w_down, (const void*)h, (const void*)saved, (const void*)y})
+        if (!aligned16(q)) return FNX_EALIGN;
+    if (ld_x % 8) return FNX_EALIGN;
+    cudaStream_t st = (cudaStream_t)stream;
+    FfnParams p;
+    memset(&p, 0, sizeof p);
+    rc = ffn_map(&p.ta, x, H, M, ld_x, 64, 128);
+    if (!rc) rc = ffn_map(&p.tb, w_gu, H, 2LL * I, H, 64, 128);
+    if (!rc) rc = ffn_map(&p.tc, h, I, M, I, 64, 32);
+    if (rc) return rc;
+    p.gu = (float*)saved;
+    p.M = M; p.N = I; p.K = H;
+    rc = ffn_launch<0, 0, FF_GATED>(p, st);
+    if (rc || !y) return rc;
+    return ffn_gemm<0, 0>(h, I, w_down, I, y, O, M, O, I, st);
+}
+
+FNX_API int fnx_gated_ffn_backward(const void* dy, long long ld_dy, const void* x, long long ld_x, const void* w_gu,
+                                   const void* w_down, const void* h, const void* saved, void* dgu, void* dx,
+                                   void* dw_gu, void* dw_down, int M, int H, int I, int O, void* stream) {
+    int rc = ffn_check(M, H, I, O);
+    if (rc) return rc;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (M == 0) {                                     // no rows: the weight gradients are zero
+        if ((dw_gu && cudaMemsetAsync(dw_gu, 0, 4ull * I * H, st) != cudaSuccess) ||
+            (dw_down && cudaMemsetAsync(dw_down, 0, 2ull * O * I, st) != cudaSuccess))
+            return FNX_ELAUNCH;
+        return FNX_OK;
+    }
+    if (!dy || !w_down || !saved || !dgu || (dx && !w_gu) || (dw_gu && !x) || (dw_down && !h) || ld_dy < O || ld_x < H)
+        return FNX_EARG;
+    for (const void* q : {dy, x, w_gu, w_down, h, saved, (const void*)dgu, (const void*)dx, (const void*)dw_gu,
+                          (const void*)dw_down})
+        if (!aligned16(q)) return FNX_EALIGN;
+    if (ld_dy % 8 || ld_x % 8) return FNX_EALIGN;
+    FfnParams p;
+    memset(&p, 0, sizeof p);
+    rc = ffn_map(&p.ta, dy, O, M, ld_dy, 64, 128);
+    if (!rc) rc = ffn_map(&p.tb, w_down, I, O, I, 64, 64);
+    if (!rc) rc = ffn_map(&p.tc, dgu, I, M, 2LL * I, 64, 32);
+    if (!rc) rc = ffn_map(&p.tc2, (const bf16*)dgu + I, I, M, 2LL * I, 64, 32);
+    if (rc) return rc;
+    p.gu = (float*)const_cast<void*>(saved);
+    p.M = M; p.N = I; p.K = O;
+    rc = ffn_launch<0, 1, FF_DGATE>(p, st);
+    if (!rc && dw_down) rc = ffn_gemm<1, 1>(dy, ld_dy, h, I, dw_down, I, O, I, M, st);
+    if (!rc && dx) rc = ffn_gemm<0, 1>(dgu, 2LL * I, w_gu, H, dx, H, M, H, 2 * I, st);
+    if (!rc && dw_gu) rc = ffn_gemm<1, 1>(dgu, 2LL * I, x, ld_x, dw_gu, H, 2 * I, H, M, st);
+    return rc;
 }
 
 // ======================================================================== dense W4

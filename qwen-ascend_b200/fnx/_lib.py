@@ -80,6 +80,9 @@ SIGNATURES = {
     "fnx_w8a16_gemm_workspace": ([I] * 4, SZ),
     "fnx_w8a16_gemm_ws": ([P] * 4 + [I] * 4 + [P, SZ, P], I),
     "fnx_w4a16_gemv": ([P, LL, P, P, P] + [I] * 4 + [P], I),
+    "fnx_gated_ffn_saved_bytes": ([I, I], SZ),
+    "fnx_gated_ffn": ([P, LL, P, P, P, P, P, I, I, I, I, P], I),
+    "fnx_gated_ffn_backward": ([P, LL, P, LL] + [P] * 8 + [I] * 4 + [P], I),
     "fnx_bf16_gemm_nt": ([P, LL, P, P, LL, I, I, I, P], I),
     "fnx_moe_decode_workspace": ([I] * 5, SZ),
     "fnx_moe_decode_w4": ([P] * 10 + [I] * 5 + [P, SZ, P], I),
