@@ -15,6 +15,7 @@
 #include "kernels_decode2.cuh"
 #include "kernels_ep.cuh"
 #include "kernels_ffn.cuh"
+#include "kernels_ffn_small.cuh"
 #include "kernels_gemm.cuh"
 #include "kernels_gemm_pair.cuh"
 #include "kernels_gemm_bf16.cuh"
@@ -274,6 +275,11 @@ int gemm_check(int mode, int epi, const GemmParams& p) {
     if (p.ld_act % 8 || !aligned16(p.act) || !aligned16(p.w) || (p.scales && !aligned16(p.scales))) return FNX_EALIGN;
     if (p.row_index && p.index_div < 1) return FNX_EARG;
     return FNX_OK;
+}
+
+int env_int(const char* name, int dflt) {
+    const char* e = getenv(name);
+    return e && *e ? atoi(e) : dflt;
 }
 
 size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
@@ -1182,18 +1188,99 @@ int ffn_launch(const FfnParams& p, cudaStream_t st) {
     return launch_rc();
 }
 
-// C [M, N] = A B^T; a, b: the stored matrices, K-major [M, K] / [N, K] or (amn, bmn) MN-major [K, M] / [K, N]
-template <int AMN, int BMN>
-int ffn_gemm(const void* a, long long lda, const void* b, long long ldb, void* c, long long ldc, int M, int N, int K,
-             cudaStream_t st) {
+// One product of the block.  a, b: the stored operands, K-major [M, K] / [N, K] or (amn, bmn) MN-major
+// [K, M] / [K, N], rows lda / ldb apart; for FF_GATED b is [2N, K].  c: C [M, N], h, or dg with du at c2.
+struct FfnGemm {
+    const void *a, *b;
+    void *c, *c2;
+    long long lda, ldb, ldc;
+    float* gu;
+    int M, N, K;
+    bool b_early;                    // b is a weight: nothing in this chain of launches writes it
+    bool chained;                    // follows another product of the chain on the stream
+};
+
+template <int AMN, int BMN, int EPI>
+int ffn_pair(const FfnGemm& g, cudaStream_t st) {
     FfnParams p;
     memset(&p, 0, sizeof p);
-    int rc = AMN ? ffn_map(&p.ta, a, M, K, lda, 64, 64) : ffn_map(&p.ta, a, K, M, lda, 64, 128);
-    if (!rc) rc = BMN ? ffn_map(&p.tb, b, N, K, ldb, 64, 64) : ffn_map(&p.tb, b, K, N, ldb, 64, 128);
-    if (!rc) rc = ffn_map(&p.tc, c, N, M, ldc, 64, 32);
+    int rc = AMN ? ffn_map(&p.ta, g.a, g.M, g.K, g.lda, 64, 64) : ffn_map(&p.ta, g.a, g.K, g.M, g.lda, 64, 128);
+    const long long nrows = EPI == FF_GATED ? 2LL * g.N : g.N;
+    if (!rc) rc = BMN ? ffn_map(&p.tb, g.b, g.N, g.K, g.ldb, 64, 64) : ffn_map(&p.tb, g.b, g.K, nrows, g.ldb, 64, 128);
+    if (!rc) rc = ffn_map(&p.tc, g.c, g.N, g.M, g.ldc, 64, 32);
+    if (!rc && EPI == FF_DGATE) rc = ffn_map(&p.tc2, g.c2, g.N, g.M, g.ldc, 64, 32);
     if (rc) return rc;
-    p.M = M; p.N = N; p.K = K;
-    return ffn_launch<AMN, BMN, FF_PLAIN>(p, st);
+    p.gu = g.gu;
+    p.M = g.M; p.N = g.N; p.K = g.K;
+    return ffn_launch<AMN, BMN, EPI>(p, st);
+}
+
+template <int AMN, int BMN, int EPI, int BN>
+int ffn_small_launch(const FfnGemm& g, int CL, int stages, cudaStream_t st) {
+    FfnSmallParams p;
+    memset(&p, 0, sizeof p);
+    int a_rows = 128;
+    if (!AMN)
+        while (a_rows > 16 && a_rows / 2 >= g.M) a_rows /= 2;
+    int rc = AMN ? ffn_map(&p.ta, g.a, g.M, g.K, g.lda, 64, 64) : ffn_map(&p.ta, g.a, g.K, g.M, g.lda, 64, a_rows);
+    const long long nrows = EPI == FF_GATED ? 2LL * g.N : g.N;
+    if (!rc) rc = BMN ? ffn_map(&p.tb, g.b, g.N, g.K, g.ldb, 64, 64) : ffn_map(&p.tb, g.b, g.K, nrows, g.ldb, 64, BN / 2);
+    if (rc) return rc;
+    p.c = (bf16*)g.c; p.c2 = (bf16*)g.c2; p.ldc = g.ldc; p.gu = g.gu;
+    p.M = g.M; p.N = g.N; p.K = g.K;
+    p.a_rows = a_rows;
+    p.b_early = g.b_early;
+    p.stages = stages;
+    const size_t smem = 1024 + ffn_small_body(BN, a_rows, stages) + sizeof(FfnSmallSmem);
+    static bool configured[FNX_MAX_DEVICES] = {};
+    const int dev = current_device();
+    if (!configured[dev]) {
+        if (cudaFuncSetAttribute(ffn_small_kernel<AMN, BMN, EPI, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 227 * 1024) != cudaSuccess)
+            return FNX_ELAUNCH;
+        configured[dev] = true;
+    }
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)CL;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    const int cols = EPI == FF_GATED ? BN / 2 : BN;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)CL, (unsigned)((g.N + cols - 1) / cols), (unsigned)((g.M + 127) / 128));
+    cfg.blockDim = dim3(FS_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = g.chained ? 2 : 1;
+    if (cudaLaunchKernelEx(&cfg, ffn_small_kernel<AMN, BMN, EPI, BN>, p) != cudaSuccess) return FNX_ELAUNCH;
+    return launch_rc();
+}
+
+template <int AMN, int BMN, int EPI>
+int ffn_product(const FfnGemm& g, cudaStream_t st) {
+    const int cols = EPI == FF_GATED ? 128 : 256, KB = (g.K + FF_BK - 1) / FF_BK;
+    const long long big = (long long)((g.M + FF_BM - 1) / FF_BM) * ((g.N + cols - 1) / cols);
+    static const int mode = env_int("FNX_FFN_SMALL", -1);
+    if (mode == 0 || (mode < 0 && big * 2 > num_sms() / 2)) return ffn_pair<AMN, BMN, EPI>(g, st);
+    // parts of K so that the tiles fill the SMs, at least two k-blocks each
+    static const int bn_env = env_int("FNX_FFN_BN", 0), cl_env = env_int("FNX_FFN_CL", 0), kb_env = env_int("FNX_FFN_KB", 92);
+    const int width = EPI == FF_GATED ? 2 : 1;
+    const long long mt = (g.M + 127) / 128;
+    const int BN = bn_env ? bn_env : mt * (((long long)g.N * width + 63) / 64) * 8 <= 2LL * num_sms() ? 64 : 128;
+    const long long tiles = mt * (((long long)g.N * width + BN - 1) / BN);
+    int CL = 1;
+    while (CL < 8 && tiles * CL < num_sms() && KB / (2 * CL) >= 2) CL *= 2;
+    if (cl_env) CL = cl_env;
+    const int per = (KB + CL - 1) / CL, a_rows = AMN || g.M > 64 ? 128 : g.M > 32 ? 64 : g.M > 16 ? 32 : 16;
+    int stages = kb_env * 1024 / ((a_rows + BN) * 128);
+    if (stages > FS_MAX_STAGES) stages = FS_MAX_STAGES;
+    if (stages > per) stages = per;
+    if (stages < 1) stages = 1;
+    if (BN == 64) return ffn_small_launch<AMN, BMN, EPI, 64>(g, CL, stages, st);
+    return ffn_small_launch<AMN, BMN, EPI, 128>(g, CL, stages, st);
 }
 
 int ffn_check(int M, int H, int I, int O) {
@@ -1218,17 +1305,11 @@ FNX_API int fnx_gated_ffn(const void* x, long long ld_x, const void* w_gu, const
         if (!aligned16(q)) return FNX_EALIGN;
     if (ld_x % 8) return FNX_EALIGN;
     cudaStream_t st = (cudaStream_t)stream;
-    FfnParams p;
-    memset(&p, 0, sizeof p);
-    rc = ffn_map(&p.ta, x, H, M, ld_x, 64, 128);
-    if (!rc) rc = ffn_map(&p.tb, w_gu, H, 2LL * I, H, 64, 128);
-    if (!rc) rc = ffn_map(&p.tc, h, I, M, I, 64, 32);
-    if (rc) return rc;
-    p.gu = (float*)saved;
-    p.M = M; p.N = I; p.K = H;
-    rc = ffn_launch<0, 0, FF_GATED>(p, st);
+    const FfnGemm gu{x, w_gu, h, nullptr, ld_x, H, I, (float*)saved, M, I, H, true, false};
+    rc = ffn_product<0, 0, FF_GATED>(gu, st);
     if (rc || !y) return rc;
-    return ffn_gemm<0, 0>(h, I, w_down, I, y, O, M, O, I, st);
+    const FfnGemm down{h, w_down, y, nullptr, I, I, O, nullptr, M, O, I, true, true};
+    return ffn_product<0, 0, FF_PLAIN>(down, st);
 }
 
 FNX_API int fnx_gated_ffn_backward(const void* dy, long long ld_dy, const void* x, long long ld_x, const void* w_gu,
@@ -1249,19 +1330,15 @@ FNX_API int fnx_gated_ffn_backward(const void* dy, long long ld_dy, const void* 
                           (const void*)dw_down})
         if (!aligned16(q)) return FNX_EALIGN;
     if (ld_dy % 8 || ld_x % 8) return FNX_EALIGN;
-    FfnParams p;
-    memset(&p, 0, sizeof p);
-    rc = ffn_map(&p.ta, dy, O, M, ld_dy, 64, 128);
-    if (!rc) rc = ffn_map(&p.tb, w_down, I, O, I, 64, 64);
-    if (!rc) rc = ffn_map(&p.tc, dgu, I, M, 2LL * I, 64, 32);
-    if (!rc) rc = ffn_map(&p.tc2, (const bf16*)dgu + I, I, M, 2LL * I, 64, 32);
-    if (rc) return rc;
-    p.gu = (float*)const_cast<void*>(saved);
-    p.M = M; p.N = I; p.K = O;
-    rc = ffn_launch<0, 1, FF_DGATE>(p, st);
-    if (!rc && dw_down) rc = ffn_gemm<1, 1>(dy, ld_dy, h, I, dw_down, I, O, I, M, st);
-    if (!rc && dx) rc = ffn_gemm<0, 1>(dgu, 2LL * I, w_gu, H, dx, H, M, H, 2 * I, st);
-    if (!rc && dw_gu) rc = ffn_gemm<1, 1>(dgu, 2LL * I, x, ld_x, dw_gu, H, 2 * I, H, M, st);
+    const FfnGemm dh{dy, w_down, dgu, (bf16*)dgu + I, ld_dy, I, 2LL * I, (float*)const_cast<void*>(saved), M, I, O, true,
+                     false};
+    const FfnGemm wd{dy, h, dw_down, nullptr, ld_dy, I, I, nullptr, O, I, M, true, true};
+    const FfnGemm gx{dgu, w_gu, dx, nullptr, 2LL * I, H, H, nullptr, M, H, 2 * I, true, true};
+    const FfnGemm wg{dgu, x, dw_gu, nullptr, 2LL * I, ld_x, H, nullptr, 2 * I, H, M, true, true};
+    rc = ffn_product<0, 1, FF_DGATE>(dh, st);
+    if (!rc && dw_down) rc = ffn_product<1, 1, FF_PLAIN>(wd, st);
+    if (!rc && dx) rc = ffn_product<0, 1, FF_PLAIN>(gx, st);
+    if (!rc && dw_gu) rc = ffn_product<1, 1, FF_PLAIN>(wg, st);
     return rc;
 }
 
@@ -1358,10 +1435,6 @@ bool decode_v1() {
     return v == 1;
 }
 
-int env_int(const char* name, int dflt) {
-    const char* e = getenv(name);
-    return e && *e ? atoi(e) : dflt;
-}
 
 DecodeLayout decode_layout(int M, int H, int I, int E, int k) {
     DecodeLayout L{};

@@ -1,0 +1,231 @@
+// The products of the gated feed-forward block (kernels_ffn.cuh) where the 256 x 256 tiles of a CTA
+// pair are too few for the 148 SMs: decode batches, short training batches, narrow blocks.  One CTA
+// takes a 128 x BN tile and one part of K; the CTAs of a cluster hold the parts of one tile and add
+// their fp32 accumulators through distributed shared memory in rank order (deterministic, no
+// workspace) before the epilogue, which the ranks share.
+//
+// Bound: at few rows the weights' bytes (BN rows of 128 bytes per k-block and CTA through a ring of TMA
+// copies as deep as shared memory allows); at more rows the latency of the chain of copies, products
+// and the cluster's sum.  Rows of A that do not exist are not loaded: the box holds p.a_rows (a power
+// of two >= M) and the tensor core multiplies whatever lies behind it into rows that are not stored.
+// A launch is a programmatic dependent of the product before it on the stream: its weights (operands
+// that no kernel of the chain writes, p.b_early) stream in while that one finishes, the rest waits.
+#pragma once
+#include "kernels_ffn.cuh"
+
+namespace fnx {
+
+constexpr int FS_THREADS = 192;
+constexpr int FS_MAX_STAGES = 16;
+
+struct FfnSmallParams {
+    CUtensorMap ta, tb;              // box {64, a_rows} / {64, BN/2} K-major, {64, 64} MN-major
+    bf16 *c, *c2;                    // C; h; dg and du
+    long long ldc;
+    float* gu;
+    int M, N, K, a_rows, stages, b_early;
+};
+
+struct FfnSmallSmem {
+    uint64_t full[FS_MAX_STAGES], empty[FS_MAX_STAGES], done;
+    uint32_t tmem_base;
+    volatile int abort;
+};
+
+FNX_DEV float4 ld_cluster_f4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+FNX_DEV void st_bf16x4(bf16* p, float a, float b, float c, float d) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf2(a, b), pack_bf2(c, d));
+}
+
+// shared memory: the ring (the sums reuse it), 16 KB that the products may read behind the last stage
+__host__ __device__ inline size_t ffn_small_ring(int bn, int a_rows, int stages) {
+    return (size_t)stages * (a_rows * 128 + bn * 128);
+}
+__host__ __device__ inline size_t ffn_small_body(int bn, int a_rows, int stages) {
+    const size_t ring = ffn_small_ring(bn, a_rows, stages) + 16384, sums = (size_t)128 * (bn + 4) * 4;
+    return ring > sums ? ring : sums;
+}
+
+template <int AMN, int BMN, int EPI, int BN>
+__global__ void __launch_bounds__(FS_THREADS) ffn_small_kernel(const __grid_constant__ FfnSmallParams p) {
+    constexpr int COLS = EPI == FF_GATED ? BN / 2 : BN;      // columns of the output per tile
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    FfnSmallSmem& S = *reinterpret_cast<FfnSmallSmem*>(base + ffn_small_body(BN, p.a_rows, p.stages));
+    float* sums = reinterpret_cast<float*>(base);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int CL = gridDim.x, rank = blockIdx.x;             // the cluster is the grid's x
+    const int n = blockIdx.y, m0 = blockIdx.z * 128;
+    const int rows = min(128, p.M - m0);
+    const int KB = (p.K + FF_BK - 1) / FF_BK;
+    const int kb0 = KB * rank / CL, kb1 = KB * (rank + 1) / CL;
+    const int a_bytes = p.a_rows * 128, stage_bytes = a_bytes + BN * 128;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < p.stages; ++s) {
+            mbar_init(&S.full[s], 1);
+            mbar_init(&S.empty[s], 1);
+        }
+        mbar_init(&S.done, 1);
+        S.abort = 0;
+        fence_mbar_init();
+    }
+    if (warp == 1) {
+        tmem_alloc(&S.tmem_base, BN);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = S.tmem_base;
+    pdl_launch_dependents();
+
+    if (warp == 0) {
+        // ------------------------------------------------ TMA copies
+        if (lane == 0) {
+            tma_prefetch_desc(&p.ta);
+            tma_prefetch_desc(&p.tb);
+            auto load_b = [&](int s, int kb) {
+                const uint32_t b = smem_u32(base + s * stage_bytes + a_bytes);
+                const int k = kb * FF_BK;
+                if (BMN) {
+#pragma unroll
+                    for (int i = 0; i < BN / 64; ++i) tma_load_2d(b + i * 8192, &p.tb, &S.full[s], n * BN + i * 64, k);
+                } else {
+                    const int r0 = EPI == FF_GATED ? n * COLS : n * BN;
+                    tma_load_2d(b, &p.tb, &S.full[s], k, r0);
+                    tma_load_2d(b + BN * 64, &p.tb, &S.full[s], k, EPI == FF_GATED ? p.N + r0 : r0 + BN / 2);
+                }
+            };
+            auto load_a = [&](int s, int kb) {
+                const uint32_t a = smem_u32(base + s * stage_bytes);
+                const int k = kb * FF_BK;
+                if (AMN) {
+                    tma_load_2d(a, &p.ta, &S.full[s], m0, k);
+                    tma_load_2d(a + 8192, &p.ta, &S.full[s], m0 + 64, k);
+                } else {
+                    tma_load_2d(a, &p.ta, &S.full[s], k, m0);
+                }
+            };
+            if (!p.b_early) pdl_wait();
+            const int first = min(kb1 - kb0, p.stages);
+            for (int j = 0; j < first; ++j) {
+                mbar_arrive_expect_tx(&S.full[j], stage_bytes);
+                load_b(j, kb0 + j);
+                if (!p.b_early) load_a(j, kb0 + j);
+            }
+            if (p.b_early) {
+                pdl_wait();
+                for (int j = 0; j < first; ++j) load_a(j, kb0 + j);
+            }
+            for (int j = first; j < kb1 - kb0; ++j) {
+                const int s = j % p.stages;
+                if (!mbar_wait(&S.empty[s], ((j / p.stages) & 1) ^ 1)) { S.abort = 1; break; }
+                mbar_arrive_expect_tx(&S.full[s], stage_bytes);
+                load_b(s, kb0 + j);
+                load_a(s, kb0 + j);
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // ------------------------------------------------ MMA issue
+        if (lane == 0) {
+            const uint32_t idesc = idesc_bf16_f32(128, BN) | ((uint32_t)AMN << 15) | ((uint32_t)BMN << 16);
+            for (int j = 0; j < kb1 - kb0; ++j) {
+                const int s = j % p.stages;
+                if (!mbar_wait(&S.full[s], (j / p.stages) & 1)) { S.abort = 1; break; }
+                tc_fence_after();
+                const uint32_t a0 = smem_u32(base + s * stage_bytes), b0 = a0 + a_bytes;
+#pragma unroll
+                for (int kk = 0; kk < FF_BK / 16; ++kk)
+                    umma_bf16(tmem, AMN ? sdesc_mnmajor_sw128(a0 + kk * 2048) : sdesc_kmajor_sw128(a0 + kk * 32),
+                              BMN ? sdesc_mnmajor_sw128(b0 + kk * 2048) : sdesc_kmajor_sw128(b0 + kk * 32), idesc,
+                              (j | kk) ? 1u : 0u);
+                umma_commit(&S.empty[s]);
+            }
+            umma_commit(&S.done);
+        }
+        __syncwarp();
+    } else {
+        // ------------------------------------------------ this part's accumulators -> shared memory
+        pdl_wait();
+        const bool ok = mbar_wait(&S.done, 0);
+        if (!__all_sync(0xffffffffu, ok)) S.abort = 1;
+        tc_fence_after();
+        const int q = warp & 3, row = q * 32 + lane;
+        if (q * 32 < rows) {
+            float* o = sums + (size_t)row * (BN + 4);
+#pragma unroll
+            for (int c0 = 0; c0 < BN; c0 += 32) {
+                uint32_t v[32];
+                tmem_ld32(tmem + ((uint32_t)(q * 32) << 16) + c0, v);
+                tmem_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    *reinterpret_cast<uint4*>(o + c0 + 4 * e) = make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+            }
+        }
+        tc_fence_before();
+    }
+    // after a wait that expired: time for the copies and products in flight to end
+    if (S.abort)
+        for (int i = 0; i < 200; ++i) __nanosleep(1000);
+    __syncthreads();
+    if (CL > 1) cluster_sync_all();
+
+    // ---------------------------------------------------- the ranks' shares of the tile
+    if (warp < 2) pdl_wait();
+    constexpr int C4 = COLS / 4;
+    const int cells = rows * C4, per = (cells + CL - 1) / CL;
+    const int cols4 = 2 * p.N / 4;
+    for (int i = rank * per + threadIdx.x; i < min(cells, (rank + 1) * per); i += FS_THREADS) {
+        const int r = i / C4, c = (i - r * C4) * 4, col = n * COLS + c;
+        if (col >= p.N) continue;
+        const float* src = sums + (size_t)r * (BN + 4) + c;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f), w = v;
+        for (int k = 0; k < CL; ++k) {
+            const float4 a = CL > 1 ? ld_cluster_f4(mapa_rank(src, k)) : *reinterpret_cast<const float4*>(src);
+            v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
+            if (EPI == FF_GATED) {
+                const float4 b = CL > 1 ? ld_cluster_f4(mapa_rank(src + COLS, k)) : *reinterpret_cast<const float4*>(src + COLS);
+                w.x += b.x; w.y += b.y; w.z += b.z; w.w += b.w;
+            }
+        }
+        const long long row = m0 + r;
+        if (EPI == FF_PLAIN) {
+            st_bf16x4(p.c + row * p.ldc + col, v.x, v.y, v.z, v.w);
+        } else if (EPI == FF_GATED) {
+            if (p.gu) {
+                reinterpret_cast<float4*>(p.gu)[ffn_gu_index((int)row, col / 4, cols4)] = v;
+                reinterpret_cast<float4*>(p.gu)[ffn_gu_index((int)row, cols4 / 2 + col / 4, cols4)] = w;
+            }
+            st_bf16x4(p.c + row * p.ldc + col, v.x * fast_sigmoid(v.x) * w.x, v.y * fast_sigmoid(v.y) * w.y,
+                      v.z * fast_sigmoid(v.z) * w.z, v.w * fast_sigmoid(v.w) * w.w);
+        } else {
+            const float4 g4 = reinterpret_cast<const float4*>(p.gu)[ffn_gu_index((int)row, col / 4, cols4)];
+            const float4 u4 = reinterpret_cast<const float4*>(p.gu)[ffn_gu_index((int)row, cols4 / 2 + col / 4, cols4)];
+            const float g[4] = {g4.x, g4.y, g4.z, g4.w}, u[4] = {u4.x, u4.y, u4.z, u4.w}, dh[4] = {v.x, v.y, v.z, v.w};
+            float dg[4], du[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float s = fast_sigmoid(g[e]);
+                dg[e] = dh[e] * u[e] * s * (1.0f + g[e] * (1.0f - s));
+                du[e] = dh[e] * g[e] * s;
+            }
+            st_bf16x4(p.c + row * p.ldc + col, dg[0], dg[1], dg[2], dg[3]);
+            st_bf16x4(p.c2 + row * p.ldc + col, du[0], du[1], du[2], du[3]);
+        }
+    }
+    if (CL > 1) cluster_sync_all();                          // every part stays until all ranks have read it
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, BN);
+    }
+}
+
+}  // namespace fnx
