@@ -1144,9 +1144,10 @@ FNX_API int fnx_bf16_gemm_nt(const void* x, long long ld_x, const void* w, void*
 
 // ======================================================================== gated feed-forward block
 namespace {
-// A bf16 matrix as an operand or output of ffn_gemm_kernel: `cols` contiguous elements per row, rows
-// `ld` elements apart.  Encoded per call (no cache: half a microsecond of host time).
-int ffn_map(CUtensorMap* out, const void* ptr, long long cols, long long rows, long long ld, unsigned b0, unsigned b1) {
+// A bf16 matrix as an operand or output of the block's products: `cols` contiguous elements per row,
+// rows `ld` elements apart.  Encoded per call (no cache: half a microsecond of host time).
+int ffn_map(CUtensorMap* out, const void* ptr, long long cols, long long rows, long long ld, unsigned b0,
+            unsigned b1) {
     EncodeTiledFn fn = encode_fn();
     if (!fn) return FNX_EDRIVER;
     const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
@@ -1158,88 +1159,116 @@ int ffn_map(CUtensorMap* out, const void* ptr, long long cols, long long rows, l
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? FNX_OK : FNX_EALIGN;
 }
 
-template <int AMN, int BMN, int EPI>
-int ffn_launch(const FfnParams& p, cudaStream_t st) {
-    const size_t smem = ffn_gemm_smem();
-    static int clusters_of[FNX_MAX_DEVICES] = {};
-    int& clusters = clusters_of[current_device()];
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 2;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.blockDim = dim3(FF_THREADS);
-    cfg.dynamicSmemBytes = smem;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    if (!clusters) {
-        if (cudaFuncSetAttribute(ffn_gemm_kernel<AMN, BMN, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 (int)smem) != cudaSuccess)
-            return FNX_ELAUNCH;
-        clusters = num_sms() / 2;
-    }
-    const int cols = EPI == FF_GATED ? 128 : 256;
-    const long long tiles = (long long)((p.M + FF_BM - 1) / FF_BM) * ((p.N + cols - 1) / cols);
-    if (tiles > 0x7fffffffLL) return FNX_ESHAPE;
-    cfg.gridDim = dim3((unsigned)(2 * (tiles < clusters ? tiles : clusters)));
-    cfg.stream = st;
-    if (cudaLaunchKernelEx(&cfg, ffn_gemm_kernel<AMN, BMN, EPI>, p) != cudaSuccess) return FNX_ELAUNCH;
-    return launch_rc();
-}
-
 // One product of the block.  a, b: the stored operands, K-major [M, K] / [N, K] or (amn, bmn) MN-major
 // [K, M] / [K, N], rows lda / ldb apart; for FF_GATED b is [2N, K].  c: C [M, N], h, or dg with du at c2.
 struct FfnGemm {
     const void *a, *b;
     void *c, *c2;
     long long lda, ldb, ldc;
-    float* gu;
     int M, N, K;
-    bool b_early;                    // b is a weight: nothing in this chain of launches writes it
-    bool chained;                    // follows another product of the chain on the stream
+    int amn, bmn;
 };
 
-template <int AMN, int BMN, int EPI>
-int ffn_pair(const FfnGemm& g, cudaStream_t st) {
-    FfnParams p;
-    memset(&p, 0, sizeof p);
-    int rc = AMN ? ffn_map(&p.ta, g.a, g.M, g.K, g.lda, 64, 64) : ffn_map(&p.ta, g.a, g.K, g.M, g.lda, 64, 128);
-    const long long nrows = EPI == FF_GATED ? 2LL * g.N : g.N;
-    if (!rc) rc = BMN ? ffn_map(&p.tb, g.b, g.N, g.K, g.ldb, 64, 64) : ffn_map(&p.tb, g.b, g.K, nrows, g.ldb, 64, 128);
-    if (!rc) rc = ffn_map(&p.tc, g.c, g.N, g.M, g.ldc, 64, 32);
-    if (!rc && EPI == FF_DGATE) rc = ffn_map(&p.tc2, g.c2, g.N, g.M, g.ldc, 64, 32);
+int ffn_maps(const FfnGemm& g, int epi, CUtensorMap* ta, CUtensorMap* tb, int a_rows, int b_rows) {
+    const int rc = g.amn ? ffn_map(ta, g.a, g.M, g.K, g.lda, 64, 64) : ffn_map(ta, g.a, g.K, g.M, g.lda, 64, a_rows);
     if (rc) return rc;
-    p.gu = g.gu;
-    p.M = g.M; p.N = g.N; p.K = g.K;
-    return ffn_launch<AMN, BMN, EPI>(p, st);
+    return g.bmn ? ffn_map(tb, g.b, g.N, g.K, g.ldb, 64, 64)
+                 : ffn_map(tb, g.b, g.K, epi == FF_GATED ? 2LL * g.N : g.N, g.ldb, 64, b_rows);
 }
 
-template <int AMN, int BMN, int EPI, int BN>
-int ffn_small_launch(const FfnGemm& g, int CL, int stages, cudaStream_t st) {
-    FfnSmallParams p;
-    memset(&p, 0, sizeof p);
-    int a_rows = 128;
-    if (!AMN)
-        while (a_rows > 16 && a_rows / 2 >= g.M) a_rows /= 2;
-    int rc = AMN ? ffn_map(&p.ta, g.a, g.M, g.K, g.lda, 64, 64) : ffn_map(&p.ta, g.a, g.K, g.M, g.lda, 64, a_rows);
-    const long long nrows = EPI == FF_GATED ? 2LL * g.N : g.N;
-    if (!rc) rc = BMN ? ffn_map(&p.tb, g.b, g.N, g.K, g.ldb, 64, 64) : ffn_map(&p.tb, g.b, g.K, nrows, g.ldb, 64, BN / 2);
-    if (rc) return rc;
-    p.c = (bf16*)g.c; p.c2 = (bf16*)g.c2; p.ldc = g.ldc; p.gu = g.gu;
-    p.M = g.M; p.N = g.N; p.K = g.K;
-    p.a_rows = a_rows;
-    p.b_early = g.b_early;
-    p.stages = stages;
-    const size_t smem = 1024 + ffn_small_body(BN, a_rows, stages) + sizeof(FfnSmallSmem);
+// Columns per tile of a product on CTA pairs: the width whose waves of tiles cost least.
+int ffn_pair_width(const FfnGemm& g, int epi, int pairs) {
+    const long long mt = (g.M + FF_BM - 1) / FF_BM;
+    int best = 256;
+    double cost = 1e30;
+    for (int bn = 256; bn >= 96; bn -= 32) {
+        if (g.bmn && bn % 128) continue;
+        const int cols = epi == FF_GATED ? bn / 2 : bn;
+        const long long waves = (mt * ((g.N + cols - 1) / cols) + pairs - 1) / pairs;
+        const double c = (double)waves * (bn + 256);
+        if (c < cost) cost = c, best = bn;
+    }
+    return best;
+}
+
+template <int EPI>
+int ffn_pair_launch(const FfnGemm* g, int count, float* gu, bool chained, cudaStream_t st) {
+    const size_t smem = ffn_gemm_smem(EPI);
     static bool configured[FNX_MAX_DEVICES] = {};
     const int dev = current_device();
     if (!configured[dev]) {
-        if (cudaFuncSetAttribute(ffn_small_kernel<AMN, BMN, EPI, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 227 * 1024) != cudaSuccess)
+        if (cudaFuncSetAttribute(ffn_gemm_kernel<EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
+            cudaSuccess)
             return FNX_ELAUNCH;
         configured[dev] = true;
     }
+    FfnParams p;
+    memset(&p, 0, sizeof p);
+    const int pairs = num_sms() / 2;
+    static const int bn_env = env_int("FNX_FFN_PAIR_BN", 0);
+    long long total = 0;
+    for (int i = 0; i < count; ++i) {
+        FfnProduct& q = p.q[i];
+        q.bn = bn_env && !g[i].bmn ? bn_env : count > 1 ? 256 : ffn_pair_width(g[i], EPI, pairs);
+        int rc = ffn_maps(g[i], EPI, &q.ta, &q.tb, 128, q.bn / 2);
+        if (!rc) rc = ffn_map(&q.tc, g[i].c, g[i].N, g[i].M, g[i].ldc, 64, 32);
+        if (!rc && EPI == FF_DGATE)
+            rc = ffn_map(&q.tc2, g[i].c2, g[i].N, g[i].M, g[i].ldc, 64, 32);
+        if (rc) return rc;
+        q.c = (bf16*)g[i].c; q.c2 = (bf16*)g[i].c2; q.ldc = g[i].ldc;
+        q.M = g[i].M; q.N = g[i].N; q.K = g[i].K; q.amn = g[i].amn; q.bmn = g[i].bmn;
+        const int cols = EPI == FF_GATED ? q.bn / 2 : q.bn;
+        q.mt = (q.M + FF_BM - 1) / FF_BM;
+        q.nt = (q.N + cols - 1) / cols;
+        total += (long long)q.mt * q.nt;
+    }
+    if (total > 0x3fffffffLL) return FNX_ESHAPE;
+    p.gu = gu; p.count = count; p.total = (int)total;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(2 * (total < pairs ? total : pairs)));
+    cfg.blockDim = dim3(FF_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = chained ? 2 : 1;
+    if (cudaLaunchKernelEx(&cfg, ffn_gemm_kernel<EPI>, p) != cudaSuccess) return FNX_ELAUNCH;
+    return launch_rc();
+}
+
+template <int EPI, int BN>
+int ffn_small_launch(const FfnGemm* g, int count, float* gu, int CL, int a_rows, int stages, bool chained,
+                     cudaStream_t st) {
+    static bool configured[FNX_MAX_DEVICES] = {};
+    const int dev = current_device();
+    if (!configured[dev]) {
+        if (cudaFuncSetAttribute(ffn_small_kernel<EPI, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) !=
+            cudaSuccess)
+            return FNX_ELAUNCH;
+        configured[dev] = true;
+    }
+    FfnSmallParams p;
+    memset(&p, 0, sizeof p);
+    const int cols = EPI == FF_GATED ? BN / 2 : BN;
+    long long total = 0;
+    for (int i = 0; i < count; ++i) {
+        FfnSmallProduct& q = p.q[i];
+        const int rc = ffn_maps(g[i], EPI, &q.ta, &q.tb, a_rows, BN / 2);
+        if (rc) return rc;
+        q.c = (bf16*)g[i].c; q.c2 = (bf16*)g[i].c2; q.ldc = g[i].ldc;
+        q.M = g[i].M; q.N = g[i].N; q.K = g[i].K; q.amn = g[i].amn; q.bmn = g[i].bmn;
+        q.b_early = chained;         // b is never what the product before it writes
+        q.nt = (q.N + cols - 1) / cols;
+        q.tiles = (q.M + 127) / 128 * q.nt;
+        total += q.tiles;
+    }
+    p.gu = gu; p.count = count; p.a_rows = a_rows; p.stages = stages; p.CL = CL;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = (unsigned)CL;
@@ -1247,40 +1276,52 @@ int ffn_small_launch(const FfnGemm& g, int CL, int stages, cudaStream_t st) {
     attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
-    const int cols = EPI == FF_GATED ? BN / 2 : BN;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)CL, (unsigned)((g.N + cols - 1) / cols), (unsigned)((g.M + 127) / 128));
+    cfg.gridDim = dim3((unsigned)(CL * total));
     cfg.blockDim = dim3(FS_THREADS);
-    cfg.dynamicSmemBytes = smem;
+    cfg.dynamicSmemBytes = 1024 + ffn_small_body(BN, a_rows, stages) + sizeof(FfnSmallSmem);
     cfg.stream = st;
     cfg.attrs = attr;
-    cfg.numAttrs = g.chained ? 2 : 1;
-    if (cudaLaunchKernelEx(&cfg, ffn_small_kernel<AMN, BMN, EPI, BN>, p) != cudaSuccess) return FNX_ELAUNCH;
+    cfg.numAttrs = chained ? 2 : 1;
+    if (cudaLaunchKernelEx(&cfg, ffn_small_kernel<EPI, BN>, p) != cudaSuccess) return FNX_ELAUNCH;
     return launch_rc();
 }
 
-template <int AMN, int BMN, int EPI>
-int ffn_product(const FfnGemm& g, cudaStream_t st) {
-    const int cols = EPI == FF_GATED ? 128 : 256, KB = (g.K + FF_BK - 1) / FF_BK;
-    const long long big = (long long)((g.M + FF_BM - 1) / FF_BM) * ((g.N + cols - 1) / cols);
+// `count` products (more than one: FF_PLAIN) in one launch.  chained: it follows another launch of the
+// block on the stream, which writes none of the b operands.
+template <int EPI>
+int ffn_products(const FfnGemm* g, int count, float* gu, bool chained, cudaStream_t st) {
     static const int mode = env_int("FNX_FFN_SMALL", -1);
-    if (mode == 0 || (mode < 0 && big * 2 > num_sms() / 2)) return ffn_pair<AMN, BMN, EPI>(g, st);
-    // parts of K so that the tiles fill the SMs, at least two k-blocks each
     static const int bn_env = env_int("FNX_FFN_BN", 0), cl_env = env_int("FNX_FFN_CL", 0), kb_env = env_int("FNX_FFN_KB", 92);
     const int width = EPI == FF_GATED ? 2 : 1;
-    const long long mt = (g.M + 127) / 128;
-    const int BN = bn_env ? bn_env : mt * (((long long)g.N * width + 63) / 64) * 8 <= 2LL * num_sms() ? 64 : 128;
-    const long long tiles = mt * (((long long)g.N * width + BN - 1) / BN);
+    long long big = 0, t64 = 0, t128 = 0;
+    int KB = 1 << 30, max_rows = 0, tall = 0;
+    for (int i = 0; i < count; ++i) {
+        const long long cols = (long long)g[i].N * width, mt = (g[i].M + 127) / 128;
+        big += (long long)((g[i].M + 255) / 256) * ((cols + 255) / 256);
+        t64 += mt * ((cols + 63) / 64);
+        t128 += mt * ((cols + 127) / 128);
+        const int kb = (g[i].K + FF_BK - 1) / FF_BK;
+        if (kb < KB) KB = kb;
+        const int rows = g[i].amn ? 128 : g[i].M;
+        if (rows > max_rows) max_rows = rows;
+        if (g[i].M > tall) tall = g[i].M;
+    }
+    if (mode == 0 || (mode < 0 && tall > 128 && big * 2 > num_sms() / 2))
+        return ffn_pair_launch<EPI>(g, count, gu, chained, st);
+    const int BN = bn_env ? bn_env : t64 * 8 <= 2LL * num_sms() ? 64 : 128;
+    const long long tiles = BN == 64 ? t64 : t128;
+    if (tiles > 0x7ffffffLL) return FNX_ESHAPE;
+    // parts of K so that the tiles fill the SMs, at least two k-blocks each
     int CL = 1;
-    while (CL < 8 && tiles * CL < num_sms() && KB / (2 * CL) >= 2) CL *= 2;
+    while (CL < FS_MAX_CL && tiles * CL < num_sms() && KB / (2 * CL) >= 2) CL *= 2;
     if (cl_env) CL = cl_env;
-    const int per = (KB + CL - 1) / CL, a_rows = AMN || g.M > 64 ? 128 : g.M > 32 ? 64 : g.M > 16 ? 32 : 16;
+    int a_rows = 128;
+    while (a_rows > 16 && a_rows / 2 >= max_rows) a_rows /= 2;
     int stages = kb_env * 1024 / ((a_rows + BN) * 128);
     if (stages > FS_MAX_STAGES) stages = FS_MAX_STAGES;
-    if (stages > per) stages = per;
-    if (stages < 1) stages = 1;
-    if (BN == 64) return ffn_small_launch<AMN, BMN, EPI, 64>(g, CL, stages, st);
-    return ffn_small_launch<AMN, BMN, EPI, 128>(g, CL, stages, st);
+    if (BN == 64) return ffn_small_launch<EPI, 64>(g, count, gu, CL, a_rows, stages, chained, st);
+    return ffn_small_launch<EPI, 128>(g, count, gu, CL, a_rows, stages, chained, st);
 }
 
 int ffn_check(int M, int H, int I, int O) {
@@ -1305,11 +1346,11 @@ FNX_API int fnx_gated_ffn(const void* x, long long ld_x, const void* w_gu, const
         if (!aligned16(q)) return FNX_EALIGN;
     if (ld_x % 8) return FNX_EALIGN;
     cudaStream_t st = (cudaStream_t)stream;
-    const FfnGemm gu{x, w_gu, h, nullptr, ld_x, H, I, (float*)saved, M, I, H, true, false};
-    rc = ffn_product<0, 0, FF_GATED>(gu, st);
+    const FfnGemm gu{x, w_gu, h, nullptr, ld_x, H, I, M, I, H, 0, 0};
+    rc = ffn_products<FF_GATED>(&gu, 1, (float*)saved, false, st);
     if (rc || !y) return rc;
-    const FfnGemm down{h, w_down, y, nullptr, I, I, O, nullptr, M, O, I, true, true};
-    return ffn_product<0, 0, FF_PLAIN>(down, st);
+    const FfnGemm down{h, w_down, y, nullptr, I, I, O, M, O, I, 0, 0};
+    return ffn_products<FF_PLAIN>(&down, 1, nullptr, true, st);
 }
 
 FNX_API int fnx_gated_ffn_backward(const void* dy, long long ld_dy, const void* x, long long ld_x, const void* w_gu,
@@ -1330,15 +1371,18 @@ FNX_API int fnx_gated_ffn_backward(const void* dy, long long ld_dy, const void* 
                           (const void*)dw_down})
         if (!aligned16(q)) return FNX_EALIGN;
     if (ld_dy % 8 || ld_x % 8) return FNX_EALIGN;
-    const FfnGemm dh{dy, w_down, dgu, (bf16*)dgu + I, ld_dy, I, 2LL * I, (float*)const_cast<void*>(saved), M, I, O, true,
-                     false};
-    const FfnGemm wd{dy, h, dw_down, nullptr, ld_dy, I, I, nullptr, O, I, M, true, true};
-    const FfnGemm gx{dgu, w_gu, dx, nullptr, 2LL * I, H, H, nullptr, M, H, 2 * I, true, true};
-    const FfnGemm wg{dgu, x, dw_gu, nullptr, 2LL * I, ld_x, H, nullptr, 2 * I, H, M, true, true};
-    rc = ffn_product<0, 1, FF_DGATE>(dh, st);
-    if (!rc && dw_down) rc = ffn_product<1, 1, FF_PLAIN>(wd, st);
-    if (!rc && dx) rc = ffn_product<0, 1, FF_PLAIN>(gx, st);
-    if (!rc && dw_gu) rc = ffn_product<1, 1, FF_PLAIN>(wg, st);
+    const FfnGemm dh{dy, w_down, dgu, (bf16*)dgu + I, ld_dy, I, 2LL * I, M, I, O, 0, 1};
+    rc = ffn_products<FF_DGATE>(&dh, 1, (float*)const_cast<void*>(saved), false, st);
+    if (rc) return rc;
+    // the three products that follow, in one launch, the one with the longest tiles first
+    FfnGemm g[FF_MAX_PRODUCTS];
+    int n = 0;
+    if (dx) g[n++] = FfnGemm{dgu, w_gu, dx, nullptr, 2LL * I, H, H, M, H, 2 * I, 0, 1};
+    if (dw_gu) g[n++] = FfnGemm{dgu, x, dw_gu, nullptr, 2LL * I, ld_x, H, 2 * I, H, M, 1, 1};
+    if (dw_down) g[n++] = FfnGemm{dy, h, dw_down, nullptr, ld_dy, I, I, O, I, M, 1, 1};
+    static const int grp = env_int("FNX_FFN_GROUP", 1);
+    if (!grp) { for (int i = 0; i < n && !rc; ++i) rc = ffn_products<FF_PLAIN>(g + i, 1, nullptr, true, st); return rc; }
+    if (n) rc = ffn_products<FF_PLAIN>(g, n, nullptr, true, st);
     return rc;
 }
 

@@ -11,19 +11,27 @@
 // A launch is a programmatic dependent of the product before it on the stream: its weights (operands
 // that no kernel of the chain writes, p.b_early) stream in while that one finishes, the rest waits.
 #pragma once
+#include <type_traits>
+
 #include "kernels_ffn.cuh"
 
 namespace fnx {
 
-constexpr int FS_THREADS = 192;
+constexpr int FS_THREADS = 256;      // warp 0 copies, 1 products, 2-5 drain the accumulator, all add the parts
 constexpr int FS_MAX_STAGES = 16;
+constexpr int FS_MAX_CL = 8;
 
-struct FfnSmallParams {
+struct FfnSmallProduct {
     CUtensorMap ta, tb;              // box {64, a_rows} / {64, BN/2} K-major, {64, 64} MN-major
     bf16 *c, *c2;                    // C; h; dg and du
     long long ldc;
+    int M, N, K, amn, bmn, b_early;
+    int nt, tiles;                   // column tiles, all tiles
+};
+struct FfnSmallParams {
+    FfnSmallProduct q[FF_MAX_PRODUCTS];
     float* gu;
-    int M, N, K, a_rows, stages, b_early;
+    int count, a_rows, stages, CL;   // a_rows: rows of a K-major A's box
 };
 
 struct FfnSmallSmem {
@@ -51,7 +59,7 @@ __host__ __device__ inline size_t ffn_small_body(int bn, int a_rows, int stages)
     return ring > sums ? ring : sums;
 }
 
-template <int AMN, int BMN, int EPI, int BN>
+template <int EPI, int BN>
 __global__ void __launch_bounds__(FS_THREADS) ffn_small_kernel(const __grid_constant__ FfnSmallParams p) {
     constexpr int COLS = EPI == FF_GATED ? BN / 2 : BN;      // columns of the output per tile
     extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -59,11 +67,14 @@ __global__ void __launch_bounds__(FS_THREADS) ffn_small_kernel(const __grid_cons
     FfnSmallSmem& S = *reinterpret_cast<FfnSmallSmem*>(base + ffn_small_body(BN, p.a_rows, p.stages));
     float* sums = reinterpret_cast<float*>(base);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int CL = gridDim.x, rank = blockIdx.x;             // the cluster is the grid's x
-    const int n = blockIdx.y, m0 = blockIdx.z * 128;
-    const int rows = min(128, p.M - m0);
-    const int KB = (p.K + FF_BK - 1) / FF_BK;
-    const int kb0 = KB * rank / CL, kb1 = KB * (rank + 1) / CL;
+    const int CL = p.CL, rank = blockIdx.x % CL;             // clusters of CL consecutive CTAs
+    int tile = blockIdx.x / CL, pi = 0;
+    while (pi + 1 < p.count && tile >= p.q[pi].tiles) tile -= p.q[pi++].tiles;
+    const FfnSmallProduct& q = p.q[pi];
+    const int n = tile % q.nt, m0 = tile / q.nt * 128;
+    const int rows = min(128, q.M - m0);
+    const int KB = (q.K + FF_BK - 1) / FF_BK;
+    const int kb0 = KB * rank / CL, nkb = KB * (rank + 1) / CL - kb0;
     const int a_bytes = p.a_rows * 128, stage_bytes = a_bytes + BN * 128;
 
     if (threadIdx.x == 0) {
@@ -86,88 +97,98 @@ __global__ void __launch_bounds__(FS_THREADS) ffn_small_kernel(const __grid_cons
     pdl_launch_dependents();
 
     if (warp == 0) {
-        // ------------------------------------------------ TMA copies
-        if (lane == 0) {
-            tma_prefetch_desc(&p.ta);
-            tma_prefetch_desc(&p.tb);
-            auto load_b = [&](int s, int kb) {
-                const uint32_t b = smem_u32(base + s * stage_bytes + a_bytes);
-                const int k = kb * FF_BK;
-                if (BMN) {
+        // ------------------------------------------------ TMA copies (a whole warp electing the issuer)
+        auto load_b = [&](int s, int kb) {
+            const uint32_t b = smem_u32(base + s * stage_bytes + a_bytes);
+            const int k = kb * FF_BK;
+            if (q.bmn) {
 #pragma unroll
-                    for (int i = 0; i < BN / 64; ++i) tma_load_2d(b + i * 8192, &p.tb, &S.full[s], n * BN + i * 64, k);
-                } else {
-                    const int r0 = EPI == FF_GATED ? n * COLS : n * BN;
-                    tma_load_2d(b, &p.tb, &S.full[s], k, r0);
-                    tma_load_2d(b + BN * 64, &p.tb, &S.full[s], k, EPI == FF_GATED ? p.N + r0 : r0 + BN / 2);
-                }
-            };
-            auto load_a = [&](int s, int kb) {
-                const uint32_t a = smem_u32(base + s * stage_bytes);
-                const int k = kb * FF_BK;
-                if (AMN) {
-                    tma_load_2d(a, &p.ta, &S.full[s], m0, k);
-                    tma_load_2d(a + 8192, &p.ta, &S.full[s], m0 + 64, k);
-                } else {
-                    tma_load_2d(a, &p.ta, &S.full[s], k, m0);
-                }
-            };
-            if (!p.b_early) pdl_wait();
-            const int first = min(kb1 - kb0, p.stages);
+                for (int i = 0; i < BN / 64; ++i) tma_load_2d(b + i * 8192, &q.tb, &S.full[s], n * BN + i * 64, k);
+            } else {
+                const int r0 = EPI == FF_GATED ? n * COLS : n * BN;
+                tma_load_2d(b, &q.tb, &S.full[s], k, r0);
+                tma_load_2d(b + BN * 64, &q.tb, &S.full[s], k, EPI == FF_GATED ? q.N + r0 : r0 + BN / 2);
+            }
+        };
+        auto load_a = [&](int s, int kb) {
+            const uint32_t a = smem_u32(base + s * stage_bytes);
+            const int k = kb * FF_BK;
+            if (q.amn) {
+                tma_load_2d(a, &q.ta, &S.full[s], m0, k);
+                tma_load_2d(a + 8192, &q.ta, &S.full[s], m0 + 64, k);
+            } else {
+                tma_load_2d(a, &q.ta, &S.full[s], k, m0);
+            }
+        };
+        if (!q.b_early) pdl_wait();
+        const int first = min(nkb, p.stages);
+        if (elect_one())
             for (int j = 0; j < first; ++j) {
                 mbar_arrive_expect_tx(&S.full[j], stage_bytes);
                 load_b(j, kb0 + j);
-                if (!p.b_early) load_a(j, kb0 + j);
+                if (!q.b_early) load_a(j, kb0 + j);
             }
-            if (p.b_early) {
-                pdl_wait();
+        __syncwarp();
+        if (q.b_early) {
+            pdl_wait();
+            if (elect_one())
                 for (int j = 0; j < first; ++j) load_a(j, kb0 + j);
-            }
-            for (int j = first; j < kb1 - kb0; ++j) {
-                const int s = j % p.stages;
-                if (!mbar_wait(&S.empty[s], ((j / p.stages) & 1) ^ 1)) { S.abort = 1; break; }
+            __syncwarp();
+        }
+        for (int j = first; j < nkb; ++j) {
+            const int s = j % p.stages;
+            if (!__all_sync(0xffffffffu, mbar_spin(&S.empty[s], ((j / p.stages) & 1) ^ 1))) { S.abort = 1; break; }
+            if (elect_one()) {
                 mbar_arrive_expect_tx(&S.full[s], stage_bytes);
                 load_b(s, kb0 + j);
                 load_a(s, kb0 + j);
             }
+            __syncwarp();
         }
-        __syncwarp();
     } else if (warp == 1) {
         // ------------------------------------------------ MMA issue
-        if (lane == 0) {
+        auto multiply = [&](auto amn, auto bmn) {
+            constexpr int AMN = decltype(amn)::value, BMN = decltype(bmn)::value;
             const uint32_t idesc = idesc_bf16_f32(128, BN) | ((uint32_t)AMN << 15) | ((uint32_t)BMN << 16);
-            for (int j = 0; j < kb1 - kb0; ++j) {
+            for (int j = 0; j < nkb; ++j) {
                 const int s = j % p.stages;
-                if (!mbar_wait(&S.full[s], (j / p.stages) & 1)) { S.abort = 1; break; }
+                if (!__all_sync(0xffffffffu, mbar_spin(&S.full[s], (j / p.stages) & 1))) { S.abort = 1; break; }
                 tc_fence_after();
                 const uint32_t a0 = smem_u32(base + s * stage_bytes), b0 = a0 + a_bytes;
+                if (elect_one()) {
 #pragma unroll
-                for (int kk = 0; kk < FF_BK / 16; ++kk)
-                    umma_bf16(tmem, AMN ? sdesc_mnmajor_sw128(a0 + kk * 2048) : sdesc_kmajor_sw128(a0 + kk * 32),
-                              BMN ? sdesc_mnmajor_sw128(b0 + kk * 2048) : sdesc_kmajor_sw128(b0 + kk * 32), idesc,
-                              (j | kk) ? 1u : 0u);
-                umma_commit(&S.empty[s]);
+                    for (int kk = 0; kk < FF_BK / 16; ++kk)
+                        umma_bf16(tmem, sdesc_at(sdesc_sw128_base(AMN), a0 + kk * kstep_bytes(AMN)),
+                                  sdesc_at(sdesc_sw128_base(BMN), b0 + kk * kstep_bytes(BMN)), idesc, (j | kk) ? 1u : 0u);
+                    umma_commit(&S.empty[s]);
+                }
+                __syncwarp();
             }
-            umma_commit(&S.done);
-        }
+        };
+        using zero = std::integral_constant<int, 0>;
+        using one = std::integral_constant<int, 1>;
+        if (q.amn) multiply(one{}, one{});
+        else if (q.bmn) multiply(zero{}, one{});
+        else multiply(zero{}, zero{});
+        if (elect_one()) umma_commit(&S.done);
         __syncwarp();
-    } else {
+    } else if (warp < 6) {
         // ------------------------------------------------ this part's accumulators -> shared memory
-        pdl_wait();
         const bool ok = mbar_wait(&S.done, 0);
         if (!__all_sync(0xffffffffu, ok)) S.abort = 1;
         tc_fence_after();
-        const int q = warp & 3, row = q * 32 + lane;
-        if (q * 32 < rows) {
+        const int lq = warp & 3, row = lq * 32 + lane;
+        if (lq * 32 < rows) {
             float* o = sums + (size_t)row * (BN + 4);
 #pragma unroll
             for (int c0 = 0; c0 < BN; c0 += 32) {
                 uint32_t v[32];
-                tmem_ld32(tmem + ((uint32_t)(q * 32) << 16) + c0, v);
+                tmem_ld32(tmem + ((uint32_t)(lq * 32) << 16) + c0, v);
                 tmem_ld_wait();
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                    *reinterpret_cast<uint4*>(o + c0 + 4 * e) = make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+                    *reinterpret_cast<uint4*>(o + c0 + 4 * e) =
+                        nkb ? make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]) : make_uint4(0, 0, 0, 0);
             }
         }
         tc_fence_before();
@@ -177,34 +198,44 @@ __global__ void __launch_bounds__(FS_THREADS) ffn_small_kernel(const __grid_cons
         for (int i = 0; i < 200; ++i) __nanosleep(1000);
     __syncthreads();
     if (CL > 1) cluster_sync_all();
+    pdl_wait();
 
     // ---------------------------------------------------- the ranks' shares of the tile
-    if (warp < 2) pdl_wait();
     constexpr int C4 = COLS / 4;
     const int cells = rows * C4, per = (cells + CL - 1) / CL;
-    const int cols4 = 2 * p.N / 4;
+    const int cols4 = 2 * q.N / 4;
     for (int i = rank * per + threadIdx.x; i < min(cells, (rank + 1) * per); i += FS_THREADS) {
         const int r = i / C4, c = (i - r * C4) * 4, col = n * COLS + c;
-        if (col >= p.N) continue;
+        if (col >= q.N) continue;
         const float* src = sums + (size_t)r * (BN + 4) + c;
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f), w = v;
-        for (int k = 0; k < CL; ++k) {
-            const float4 a = CL > 1 ? ld_cluster_f4(mapa_rank(src, k)) : *reinterpret_cast<const float4*>(src);
-            v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
-            if (EPI == FF_GATED) {
-                const float4 b = CL > 1 ? ld_cluster_f4(mapa_rank(src + COLS, k)) : *reinterpret_cast<const float4*>(src + COLS);
-                w.x += b.x; w.y += b.y; w.z += b.z; w.w += b.w;
-            }
+        float4 v = *reinterpret_cast<const float4*>(src), w = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (EPI == FF_GATED) w = *reinterpret_cast<const float4*>(src + COLS);
+        if (CL > 1) {
+            float4 a[FS_MAX_CL], b[FS_MAX_CL];               // all requested before the first is added
+#pragma unroll
+            for (int k = 0; k < FS_MAX_CL; ++k)
+                if (k < CL) {
+                    a[k] = ld_cluster_f4(mapa_rank(src, k));
+                    if (EPI == FF_GATED) b[k] = ld_cluster_f4(mapa_rank(src + COLS, k));
+                }
+            v = a[0];
+            if (EPI == FF_GATED) w = b[0];
+#pragma unroll
+            for (int k = 1; k < FS_MAX_CL; ++k)
+                if (k < CL) {
+                    v.x += a[k].x; v.y += a[k].y; v.z += a[k].z; v.w += a[k].w;
+                    if (EPI == FF_GATED) { w.x += b[k].x; w.y += b[k].y; w.z += b[k].z; w.w += b[k].w; }
+                }
         }
         const long long row = m0 + r;
         if (EPI == FF_PLAIN) {
-            st_bf16x4(p.c + row * p.ldc + col, v.x, v.y, v.z, v.w);
+            st_bf16x4(q.c + row * q.ldc + col, v.x, v.y, v.z, v.w);
         } else if (EPI == FF_GATED) {
             if (p.gu) {
                 reinterpret_cast<float4*>(p.gu)[ffn_gu_index((int)row, col / 4, cols4)] = v;
                 reinterpret_cast<float4*>(p.gu)[ffn_gu_index((int)row, cols4 / 2 + col / 4, cols4)] = w;
             }
-            st_bf16x4(p.c + row * p.ldc + col, v.x * fast_sigmoid(v.x) * w.x, v.y * fast_sigmoid(v.y) * w.y,
+            st_bf16x4(q.c + row * q.ldc + col, v.x * fast_sigmoid(v.x) * w.x, v.y * fast_sigmoid(v.y) * w.y,
                       v.z * fast_sigmoid(v.z) * w.z, v.w * fast_sigmoid(v.w) * w.w);
         } else {
             const float4 g4 = reinterpret_cast<const float4*>(p.gu)[ffn_gu_index((int)row, col / 4, cols4)];
@@ -217,8 +248,8 @@ __global__ void __launch_bounds__(FS_THREADS) ffn_small_kernel(const __grid_cons
                 dg[e] = dh[e] * u[e] * s * (1.0f + g[e] * (1.0f - s));
                 du[e] = dh[e] * g[e] * s;
             }
-            st_bf16x4(p.c + row * p.ldc + col, dg[0], dg[1], dg[2], dg[3]);
-            st_bf16x4(p.c2 + row * p.ldc + col, du[0], du[1], du[2], du[3]);
+            st_bf16x4(q.c + row * q.ldc + col, dg[0], dg[1], dg[2], dg[3]);
+            st_bf16x4(q.c2 + row * q.ldc + col, du[0], du[1], du[2], du[3]);
         }
     }
     if (CL > 1) cluster_sync_all();                          // every part stays until all ranks have read it
