@@ -1291,34 +1291,34 @@ int ffn_small_launch(const FfnGemm* g, int count, float* gu, int CL, int a_rows,
 // block on the stream, which writes none of the b operands.
 template <int EPI>
 int ffn_products(const FfnGemm* g, int count, float* gu, bool chained, cudaStream_t st) {
-    static const int mode = env_int("FNX_FFN_SMALL", -1);
-    static const int bn_env = env_int("FNX_FFN_BN", 0), cl_env = env_int("FNX_FFN_CL", 0), kb_env = env_int("FNX_FFN_KB", 92);
     const int width = EPI == FF_GATED ? 2 : 1;
-    long long big = 0, t64 = 0, t128 = 0;
-    int KB = 1 << 30, max_rows = 0, tall = 0;
+    long long t64 = 0, t128 = 0;
+    int KB = 1 << 30, box_rows = 0, rows = 0;
     for (int i = 0; i < count; ++i) {
         const long long cols = (long long)g[i].N * width, mt = (g[i].M + 127) / 128;
-        big += (long long)((g[i].M + 255) / 256) * ((cols + 255) / 256);
         t64 += mt * ((cols + 63) / 64);
         t128 += mt * ((cols + 127) / 128);
         const int kb = (g[i].K + FF_BK - 1) / FF_BK;
         if (kb < KB) KB = kb;
-        const int rows = g[i].amn ? 128 : g[i].M;
-        if (rows > max_rows) max_rows = rows;
-        if (g[i].M > tall) tall = g[i].M;
+        if (g[i].M > rows) rows = g[i].M;
+        if (g[i].amn) box_rows = 128;
+        else if (g[i].M > box_rows) box_rows = g[i].M;
     }
-    if (mode == 0 || (mode < 0 && tall > 128 && big * 2 > num_sms() / 2))
-        return ffn_pair_launch<EPI>(g, count, gu, chained, st);
-    const int BN = bn_env ? bn_env : t64 * 8 <= 2LL * num_sms() ? 64 : 128;
+    // Few rows: the weights' bytes are the work, 128-row tiles of them.  More rows: 64 columns, while
+    // the tiles fit the SMs twice; beyond that CTA pairs, unless their 256 rows would be half empty.
+    static const int t64_env = env_int("FNX_FFN_T64", 256);
+    const bool few = rows <= 32, fits = t64 <= t64_env;
+    if (!few && !fits && rows > 128) return ffn_pair_launch<EPI>(g, count, gu, chained, st);
+    const int BN = few || !fits ? 128 : 64;
     const long long tiles = BN == 64 ? t64 : t128;
     if (tiles > 0x7ffffffLL) return FNX_ESHAPE;
-    // parts of K so that the tiles fill the SMs, at least two k-blocks each
+    // parts of K while the CTAs fit the SMs twice, at least four k-blocks each (a part costs the
+    // cluster's sum: 2 k-blocks each took 10.2 us where 4 took 7.5, 128 x 1024 x 2048)
     int CL = 1;
-    while (CL < FS_MAX_CL && tiles * CL < num_sms() && KB / (2 * CL) >= 2) CL *= 2;
-    if (cl_env) CL = cl_env;
+    while (CL < FS_MAX_CL && 2 * CL * tiles <= 2LL * num_sms() && KB / (2 * CL) >= 4) CL *= 2;
     int a_rows = 128;
-    while (a_rows > 16 && a_rows / 2 >= max_rows) a_rows /= 2;
-    int stages = kb_env * 1024 / ((a_rows + BN) * 128);
+    while (a_rows > 16 && a_rows / 2 >= box_rows) a_rows /= 2;
+    int stages = 92 * 1024 / ((a_rows + BN) * 128);          // a ring that leaves room for a second CTA on the SM
     if (stages > FS_MAX_STAGES) stages = FS_MAX_STAGES;
     if (BN == 64) return ffn_small_launch<EPI, 64>(g, count, gu, CL, a_rows, stages, chained, st);
     return ffn_small_launch<EPI, 128>(g, count, gu, CL, a_rows, stages, chained, st);
