@@ -7,7 +7,6 @@ no fallback: if the library or a CUDA device is missing, the call raises.
 from __future__ import annotations
 
 import ctypes
-import functools
 import os
 from pathlib import Path
 
@@ -93,6 +92,8 @@ SIGNATURES = {
     "fnx_w4gemv_launch_layers": ([ctypes.POINTER(P)] * 4 + [I] * 6 + [P, P], I),
 }
 
+EALIGN = -3                     # the library's answer to a misaligned pointer or stride
+
 _lib = None
 
 
@@ -127,17 +128,10 @@ def raw_stream(device) -> int:
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
-def on_device(fn):
-    """Runs ``fn(first tensor, ...)`` with that tensor's device current, where it is not already (the
-    library launches on the current device)."""
-    @functools.wraps(fn)
-    def call(self_or_tensor, *args, **kw):
-        t = self_or_tensor if isinstance(self_or_tensor, torch.Tensor) else args[0] if args else None
-        if isinstance(t, torch.Tensor) and t.is_cuda and t.device.index != torch.cuda.current_device():
-            with torch.cuda.device(t.device):
-                return fn(self_or_tensor, *args, **kw)
-        return fn(self_or_tensor, *args, **kw)
-    return call
+def elsewhere(t) -> bool:
+    """Whether the CUDA tensor's device is not the current one.  The library launches on the current
+    device, so a caller then makes ``t.device`` current and calls itself again."""
+    return t.get_device() != torch._C._cuda_getDevice()
 
 
 def ptr(t) -> int | None:

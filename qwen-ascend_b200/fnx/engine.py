@@ -404,25 +404,28 @@ class DenseW4:
         if (self.w4.data_ptr() | self.sc.data_ptr()) % 16:
             raise ValueError("DenseW4: weights and scales must be 16-byte aligned")
         self._fn = _lib.lib().fnx_w4a16_gemv
+        self._pw, self._ps = self.w4.data_ptr(), self.sc.data_ptr()
 
     def __call__(self, x):
-        if x.shape[-1] != self.K or x.device != self.w4.device:
-            raise ValueError(f"DenseW4: rows of {self.K} on {self.w4.device} expected, got {tuple(x.shape)} on {x.device}")
-        return self._run(x)
-
-    @_lib.on_device
-    def _run(self, x):
-        x2 = x if x.dtype == BF16 else x.to(BF16)
-        if x2.dim() != 2 or x2.stride(1) != 1 or x2.stride(0) % 4 or x2.stride(0) < self.K or x2.data_ptr() % 16:
-            x2 = x2.reshape(-1, self.K).contiguous()
-            if x2.data_ptr() % 16:
-                x2 = x2.clone()
+        shape, dev, K = x.shape, self.w4.device, self.K
+        if shape[-1] != K or x.device != dev:
+            raise ValueError(f"DenseW4: rows of {K} on {dev} expected, got {tuple(shape)} on {x.device}")
+        if _lib.elsewhere(x):
+            with torch.cuda.device(dev):
+                return self(x)
+        x2 = x if x.dtype is BF16 else x.to(BF16)
+        if len(shape) != 2:
+            x2 = x2.reshape(-1, K)
         M = x2.shape[0]
-        y = torch.empty(M, self.N, dtype=BF16, device=x2.device)
-        rc = self._fn(x2.data_ptr(), x2.stride(0) if M > 1 else self.K, self.w4.data_ptr(), self.sc.data_ptr(),
-                      y.data_ptr(), M, self.K, self.N, self.gs, _lib.raw_stream(x2.device))
+        ld, one = x2.stride()
+        if M < 2:
+            ld = K
+        if one != 1 or ld % 4 or ld < K or x2.data_ptr() % 16:
+            x2, ld = x2.clone(memory_format=torch.contiguous_format), K
+        y = torch.empty(M, self.N, dtype=BF16, device=dev)
+        rc = self._fn(x2.data_ptr(), ld, self._pw, self._ps, y.data_ptr(), M, K, self.N, self.gs, _lib.raw_stream(dev))
         _lib.check(rc, "W4A16 GEMV")
-        return y if x.dim() == 2 else y.view(*x.shape[:-1], self.N)
+        return y if len(shape) == 2 else y.view(*shape[:-1], self.N)
 
     def deq_w(self):
         """fp32 ``[N, K]``: the weights a call multiplies with."""

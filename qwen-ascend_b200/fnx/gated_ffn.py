@@ -17,14 +17,19 @@ BF16 = torch.bfloat16
 
 def _rows(t, n, what, like):
     """``t [.., n]`` as bf16 rows the kernels can read: ``(2-D view or copy, row stride)``."""
-    if t.shape[-1] != n or t.device != like.device:
-        raise ValueError(f"GatedFFN: {what} rows of {n} on {like.device} expected, got {tuple(t.shape)} on {t.device}")
-    r = t if t.dtype == BF16 else t.to(BF16)
-    if r.dim() != 2:
-        r = r.reshape(-1, n)
-    if r.stride(1) != 1 or (r.shape[0] > 1 and (r.stride(0) % 8 or r.stride(0) < n)) or r.data_ptr() % 16:
-        r = r.clone(memory_format=torch.contiguous_format)
-    return r, r.stride(0) if r.shape[0] > 1 else n
+    shape = t.shape
+    if shape[-1] != n or t.device != like.device:
+        raise ValueError(f"GatedFFN: {what} rows of {n} on {like.device} expected, got {tuple(shape)} on {t.device}")
+    if t.dtype is not BF16:
+        t = t.to(BF16)
+    if len(shape) != 2:
+        t = t.reshape(-1, n)
+    ld, one = t.stride()
+    if t.shape[0] < 2:
+        ld = n
+    if (one != 1 and n > 1) or ld % 8 or ld < n or t.data_ptr() % 16:
+        t, ld = t.clone(memory_format=torch.contiguous_format), n
+    return t, ld
 
 
 class GatedFFN:
@@ -49,8 +54,14 @@ class GatedFFN:
         self.w_gu, self.w_down = w_gu, w_down
         self._lib = _lib.lib()
 
-    def _forward(self, x2, ld, keep, down):
-        M, dev = x2.shape[0], x2.device
+    def _forward(self, x, keep, down):
+        """``(x as rows, h, kept pre-activations, y)``."""
+        dev = self.w_gu.device
+        x2, ld = _rows(x, self.H, "input", self.w_gu)
+        if _lib.elsewhere(x2):
+            with torch.cuda.device(dev):
+                return self._forward(x, keep, down)
+        M = x2.shape[0]
         h = torch.empty(M, self.I, dtype=BF16, device=dev)
         y = torch.empty(M, self.O, dtype=BF16, device=dev) if down else None
         gu = torch.empty(self._lib.fnx_gated_ffn_saved_bytes(M, self.I), dtype=torch.uint8, device=dev) if keep else None
@@ -58,30 +69,23 @@ class GatedFFN:
                                      h.data_ptr(), _lib.ptr(gu), _lib.ptr(y), M, self.H, self.I, self.O,
                                      _lib.raw_stream(dev))
         _lib.check(rc, "gated feed-forward block")
-        return h, gu, y
+        return x2, h, gu, y
 
-    @_lib.on_device
     def __call__(self, x):
-        x2, ld = _rows(x, self.H, "input", self.w_gu)
-        y = self._forward(x2, ld, False, True)[2]
+        y = self._forward(x, False, True)[3]
         return y if x.dim() == 2 else y.view(*x.shape[:-1], self.O)
 
-    @_lib.on_device
     def gated(self, x):
         """``h = silu(x Wg^T) * (x Wu^T)``: ``[.., H] -> [.., I]``."""
-        x2, ld = _rows(x, self.H, "input", self.w_gu)
-        h = self._forward(x2, ld, False, False)[0]
+        h = self._forward(x, False, False)[1]
         return h if x.dim() == 2 else h.view(*x.shape[:-1], self.I)
 
-    @_lib.on_device
     def forward_train(self, x):
         """``(y, saved)``: ``saved`` is handed to ``backward``; it holds ``x`` itself, which must not
         be overwritten before, and ``8 * I`` bytes a row of pre-activations."""
-        x2, ld = _rows(x, self.H, "input", self.w_gu)
-        h, gu, y = self._forward(x2, ld, True, True)
+        x2, h, gu, y = self._forward(x, True, True)
         return y if x.dim() == 2 else y.view(*x.shape[:-1], self.O), (x2, h, gu, x.shape)
 
-    @_lib.on_device
     def backward(self, dy, saved, need=(True, True, True)):
         """``(dx, dw_gu, dw_down)`` in bf16, ``None`` where ``need`` is false.  May be called again
         with the same ``saved``."""
@@ -90,6 +94,9 @@ class GatedFFN:
         dy2, ld = _rows(dy, self.O, "gradient", self.w_gu)
         if dy2.shape[0] != M:
             raise ValueError(f"GatedFFN.backward: {dy2.shape[0]} rows for a forward of {M}")
+        if _lib.elsewhere(x2):
+            with torch.cuda.device(dev):
+                return self.backward(dy, saved, need)
         dgu = torch.empty(M, 2 * self.I, dtype=BF16, device=dev)
         dx = torch.empty(M, self.H, dtype=BF16, device=dev) if need[0] else None
         dw_gu = torch.empty_like(self.w_gu) if need[1] else None

@@ -15,6 +15,8 @@ import torch
 
 from . import _lib
 
+BF16 = torch.bfloat16
+
 
 def inject(hyper, gate, values):
     b = hyper.shape[0]
@@ -35,27 +37,36 @@ def inject(hyper, gate, values):
 
 
 def _inject_norm_args(hyper, gate, values, w_next, w_post):
-    """Checks shared by the two directions -> ``(b, H, HC)``."""
-    b = hyper.shape[0]
-    H = values.shape[-1]
-    if values.numel() != b * H or H < 1 or hyper.shape[-1] % H or hyper.numel() != b * hyper.shape[-1]:
-        raise ValueError(f"inject_norm: hyper {tuple(hyper.shape)} and values {tuple(values.shape)} are not "
-                         "[b, 1, HC*H] and [b, 1, H]")
-    HC = hyper.shape[-1] // H
+    """Checks shared by the two directions -> ``(b, H, HC, whether a tensor has to be packed)``."""
+    hs, vs = hyper.shape, values.shape
+    b, W, H = hs[0], hs[-1], vs[-1]
+    if H < 1 or W % H or values.numel() != b * H or hyper.numel() != b * W:
+        raise ValueError(f"inject_norm: hyper {tuple(hs)} and values {tuple(vs)} are not [b, 1, HC*H] and [b, 1, H]")
+    HC = W // H
     if H % 8 or H > 16384 or HC > 4 or (HC + 2) * H > 56000:
         raise ValueError(f"inject_norm: H={H}, HC={HC}: H must be a multiple of 8 up to 16384, HC at most 4 and "
                          "(HC + 2) * H at most 56000")
-    for name, t, n in (("gate", gate, b * HC), ("w_next", w_next, HC * H), ("w_post", w_post, H)):
-        if t is not None and t.numel() != n:
-            raise ValueError(f"inject_norm: {name} holds {t.numel()} values, {n} expected")
-    for t in (hyper, gate, values, w_next, w_post):
-        if t is not None and (t.dtype != torch.bfloat16 or t.device != hyper.device):
-            raise ValueError("inject_norm: bf16 tensors on one device expected")
-    _lib.require_cuda(hyper)
-    return b, H, HC
+    at = hyper.get_device()
+    pack = not (hyper.is_contiguous() and values.is_contiguous())
+    ok = hyper.dtype is BF16 and values.dtype is BF16 and values.get_device() == at
+    for t, n in ((gate, b * HC), (w_next, W), (w_post, H)):
+        if t is not None:
+            ok = ok and t.dtype is BF16 and t.get_device() == at and t.numel() == n
+            pack = pack or not t.is_contiguous()
+    if not ok:
+        raise ValueError(f"inject_norm: bf16 tensors on one device expected, a gate of {b * HC} values, w_next of {W}, "
+                         f"w_post of {H}")
+    if at < 0:
+        _lib.require_cuda(hyper)
+    return b, H, HC, pack
 
 
-@_lib.on_device
+def _packed(*ts):
+    """Contiguous, 16-byte aligned copies of what is not."""
+    return [t if t is None or (t.is_contiguous() and t.data_ptr() % 16 == 0)
+            else t.clone(memory_format=torch.contiguous_format) for t in ts]
+
+
 def inject_norm(hyper, gate, values, w_next=None, *, w_post=None, scale=1.0, eps=1e-6):
     """``state = hyper + scale * gate * z`` per branch with ``z = values`` (or its rms norm times
     ``1 + w_post``), and ``normed``, the rms norm of every branch of ``state`` times ``1 + w_next``
@@ -65,24 +76,29 @@ def inject_norm(hyper, gate, values, w_next=None, *, w_post=None, scale=1.0, eps
     ``w_next`` ``[HC*H]``, ``w_post`` ``[H]``; HC = 1 is an ordinary residual stream.  Returns
     ``(state, normed)`` shaped like ``hyper``.  fp32 inside, each output rounded once; ``normed``
     comes from the unrounded state, so it can differ by one rounding from a norm of ``state``."""
-    b, H, HC = _inject_norm_args(hyper, gate, values, w_next, w_post)
-    hyper, values = hyper.contiguous(), values.contiguous()
-    gate, w_next, w_post = (None if t is None else t.contiguous() for t in (gate, w_next, w_post))
+    b, H, HC, pack = _inject_norm_args(hyper, gate, values, w_next, w_post)
+    dev = hyper.device
+    if _lib.elsewhere(hyper):
+        with torch.cuda.device(dev):
+            return inject_norm(hyper, gate, values, w_next, w_post=w_post, scale=scale, eps=eps)
+    if pack:
+        hyper, gate, values, w_next, w_post = _packed(hyper, gate, values, w_next, w_post)
     state = torch.empty_like(hyper)
     normed = None if w_next is None else torch.empty_like(hyper)
-    rc = _lib.lib().fnx_inject_norm(hyper.data_ptr(), _lib.ptr(gate), values.data_ptr(), _lib.ptr(w_post),
-                                    _lib.ptr(w_next), state.data_ptr(), _lib.ptr(normed), b, H, HC, scale, eps,
-                                    _lib.stream(hyper.device))
+    ptr = _lib.ptr
+    rc = _lib.lib().fnx_inject_norm(hyper.data_ptr(), ptr(gate), values.data_ptr(), ptr(w_post), ptr(w_next),
+                                    state.data_ptr(), ptr(normed), b, H, HC, scale, eps, _lib.raw_stream(dev))
+    if rc == _lib.EALIGN and not pack:                # a view that starts off a 16-byte boundary
+        return inject_norm(*_packed(hyper, gate, values, w_next), w_post=_packed(w_post)[0], scale=scale, eps=eps)
     _lib.check(rc, "residual injection with norms")
     return state, normed
 
 
-@_lib.on_device
 def inject_norm_backward(d_state, d_normed, state, gate, values, w_next=None, *, w_post=None, scale=1.0, eps=1e-6):
     """Gradients of ``inject_norm`` from the gradients of its outputs (either may be ``None``: zero),
     the ``state`` it returned and its inputs: ``(d_hyper, d_gate, d_values, d_w_next, d_w_post)``,
     bf16 in the inputs' shapes, ``None`` where the input was ``None``.  Deterministic."""
-    b, H, HC = _inject_norm_args(state, gate, values, w_next, w_post)
+    b, H, HC, _ = _inject_norm_args(state, gate, values, w_next, w_post)
     if d_state is None and d_normed is None:
         raise ValueError("inject_norm_backward: d_state or d_normed needed")
     if d_normed is not None and w_next is None:
@@ -90,18 +106,21 @@ def inject_norm_backward(d_state, d_normed, state, gate, values, w_next=None, *,
     for t in (d_state, d_normed):
         if t is not None and (t.numel() != state.numel() or t.dtype != torch.bfloat16 or t.device != state.device):
             raise ValueError("inject_norm_backward: gradients must be bf16, shaped and placed like state")
-    d_state, d_normed, gate_c, w_next_c, w_post_c = (None if t is None else t.contiguous()
-                                                     for t in (d_state, d_normed, gate, w_next, w_post))
-    state, values_c = state.contiguous(), values.contiguous()
-    d_hyper = torch.empty_like(state)
-    new = lambda t: None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device)      # noqa: E731
-    d_gate, d_values, d_w_next, d_w_post = new(gate), new(values), new(w_next), new(w_post)
+    dev = state.device
+    if _lib.elsewhere(state):
+        with torch.cuda.device(dev):
+            return inject_norm_backward(d_state, d_normed, state, gate, values, w_next, w_post=w_post, scale=scale,
+                                        eps=eps)
+    d_state, d_normed, state, values_c, gate_c, w_next_c, w_post_c = _packed(d_state, d_normed, state, values, gate,
+                                                                             w_next, w_post)
+    new = lambda t: None if t is None else torch.empty_like(t)                                       # noqa: E731
+    d_hyper, d_gate, d_values, d_w_next, d_w_post = new(state), new(gate_c), new(values_c), new(w_next_c), new(w_post_c)
     L = _lib.lib()
     nws = L.fnx_inject_norm_backward_workspace(b, H, HC)
-    ws = torch.empty(nws, dtype=torch.uint8, device=state.device)
+    ws = torch.empty(nws, dtype=torch.uint8, device=dev)
     rc = L.fnx_inject_norm_backward(_lib.ptr(d_state), _lib.ptr(d_normed), state.data_ptr(), _lib.ptr(gate_c),
                                     values_c.data_ptr(), _lib.ptr(w_post_c), _lib.ptr(w_next_c), d_hyper.data_ptr(),
                                     _lib.ptr(d_gate), d_values.data_ptr(), _lib.ptr(d_w_post), _lib.ptr(d_w_next),
-                                    b, H, HC, scale, eps, ws.data_ptr(), nws, _lib.stream(state.device))
+                                    b, H, HC, scale, eps, ws.data_ptr(), nws, _lib.raw_stream(dev))
     _lib.check(rc, "gradient of the residual injection with norms")
     return d_hyper, d_gate, d_values, d_w_next, d_w_post

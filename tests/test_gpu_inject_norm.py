@@ -75,7 +75,7 @@ def test_forward_without_gate_or_norms_is_a_residual_add():
 
 
 def test_strided_and_two_dimensional_inputs():
-    from fnx.native_inject import inject_norm
+    from fnx.native_inject import inject_norm, inject_norm_backward
     h, g, v, wn, wp = inputs(6, 128, 4, 5)
     wide = torch.randn(6, 1, 2 * 512, device=DEV).to(BF16)
     wide[..., ::2] = h
@@ -84,6 +84,13 @@ def test_strided_and_two_dimensional_inputs():
     flat = inject_norm(h.view(6, -1), g.view(6, -1), v.view(6, -1), wn, w_post=wp)
     for w, x, y in zip(want, got, flat):
         assert torch.equal(w, x) and torch.equal(w.view(6, -1), y)
+    off = torch.empty(6 * 512 + 3, dtype=BF16, device=DEV)[3:]     # contiguous, off a 16-byte boundary
+    off.copy_(h.view(-1))
+    odd = inject_norm(off.view(6, 1, 512), g, v, wn, w_post=wp)
+    assert torch.equal(odd[0], want[0]) and torch.equal(odd[1], want[1])
+    grads = inject_norm_backward(h, h, want[0], g, v, wn, w_post=wp)
+    for a, c in zip(grads, inject_norm_backward(off.view(6, 1, 512), h, want[0], g, v, wn, w_post=wp)):
+        assert torch.equal(a, c)
 
 
 def test_empty_batch():
