@@ -417,11 +417,32 @@ int inject_norm_launch(const InjectNormParams& p, int batch, cudaStream_t st) {
     return inject_norm_launch_t<4, BR>(p, batch, st);
 }
 
-size_t inject_norm_bwd_smem(int H, int HC) { return (size_t)(HC + 2) * H * sizeof(float); }
+// the wide form: sums of the weight gradients and dz; the narrow one: two stages of a token's rows
+size_t inject_norm_bwd_smem(int H, int HC) {
+    return H <= 4096 ? (size_t)2 * (3 * HC + 1) * H * sizeof(bf16) : (size_t)(HC + 2) * H * sizeof(float);
+}
 int inject_norm_bwd_blocks(int batch, int H, int HC) {
-    const int per_sm = inject_norm_bwd_smem(H, HC) <= 100 * 1024 ? 2 : 1;
+    const int threads = H <= 4096 ? (H / 8 + 31) / 32 * 32 : 512;
+    int per_sm = (int)(220 * 1024 / (inject_norm_bwd_smem(H, HC) + 4096));       // shared memory
+    if (per_sm > 1024 / threads) per_sm = 1024 / threads;                        // registers
+    if (per_sm > 4) per_sm = 4;
+    if (per_sm < 1) per_sm = 1;
     const int g = per_sm * num_sms();
     return batch < g ? batch : g;
+}
+
+template <int HC>
+int inject_norm_bwd_launch(const InjectNormBwdParams& p, int blocks, cudaStream_t st) {
+    static bool configured[FNX_MAX_DEVICES] = {};
+    const int dev = current_device();
+    if (!configured[dev]) {
+        if (cudaFuncSetAttribute(inject_norm_bwd_kernel<HC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 (int)inject_norm_bwd_smem(4096, HC)) != cudaSuccess)
+            return FNX_ELAUNCH;
+        configured[dev] = true;
+    }
+    inject_norm_bwd_kernel<HC><<<blocks, (p.H / 8 + 31) / 32 * 32, inject_norm_bwd_smem(p.H, HC), st>>>(p);
+    return launch_rc();
 }
 }  // namespace
 
@@ -463,21 +484,27 @@ FNX_API int fnx_inject_norm_backward(const void* d_state, const void* d_normed, 
     cudaStream_t st = (cudaStream_t)stream;
     const int blocks = inject_norm_bwd_blocks(batch, H, HC);
     if (batch) {
-        static bool configured[FNX_MAX_DEVICES] = {};
-        const int dev = current_device();
-        if (!configured[dev]) {
-            if (cudaFuncSetAttribute(inject_norm_bwd_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     IN_MAX_SUMS * (int)sizeof(float)) != cudaSuccess)
-                return FNX_ELAUNCH;
-            configured[dev] = true;
-        }
         const InjectNormBwdParams p{(const bf16*)d_state, (const bf16*)d_normed, (const bf16*)state, (const bf16*)gate,
                                     (const bf16*)values, (const bf16*)w_post, (const bf16*)w_next, (bf16*)d_hyper,
                                     (bf16*)d_gate, (bf16*)d_values, (float*)ws, batch, H, HC, scale, eps};
-        int threads = (H / 8 + 31) / 32 * 32;
-        if (threads > 512) threads = 512;
-        inject_norm_bwd_kernel<<<blocks, threads, inject_norm_bwd_smem(H, HC), st>>>(p);
-        const int rc = launch_rc();
+        int rc = FNX_OK;
+        if (H <= 4096) {
+            rc = HC == 1   ? inject_norm_bwd_launch<1>(p, blocks, st)
+                 : HC == 2 ? inject_norm_bwd_launch<2>(p, blocks, st)
+                 : HC == 3 ? inject_norm_bwd_launch<3>(p, blocks, st)
+                           : inject_norm_bwd_launch<4>(p, blocks, st);
+        } else {
+            static bool configured[FNX_MAX_DEVICES] = {};
+            const int dev = current_device();
+            if (!configured[dev]) {
+                if (cudaFuncSetAttribute(inject_norm_bwd_wide_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         IN_MAX_SUMS * (int)sizeof(float)) != cudaSuccess)
+                    return FNX_ELAUNCH;
+                configured[dev] = true;
+            }
+            inject_norm_bwd_wide_kernel<<<blocks, 512, inject_norm_bwd_smem(H, HC), st>>>(p);
+            rc = launch_rc();
+        }
         if (rc) return rc;
     }
     if (d_w_next || d_w_post) {

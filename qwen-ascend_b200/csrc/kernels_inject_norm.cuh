@@ -158,9 +158,190 @@ struct InjectNormBwdParams {
     float scale, eps;
 };
 
-// Persistent blocks, tokens blockIdx.x, + gridDim.x, ...: every thread owns fixed columns, whose
-// weight-gradient sums it keeps in shared memory over all of its block's tokens.
+// Sums of 32 values per lane over a warp, value i in lane i: each step adds half of the values the
+// lane pair holds and hands the other half over (31 shuffles for all 32).
+FNX_DEV float warp_sums32(float (&v)[32]) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        const bool up = lane & o;
+#pragma unroll
+        for (int i = 0; i < o; ++i) {
+            const float mine = up ? v[i + o] : v[i], theirs = up ? v[i] : v[i + o];
+            v[i] = mine + __shfl_xor_sync(0xffffffffu, theirs, o);
+        }
+    }
+    return v[0];
+}
+
+// The backward for H <= 4096: persistent blocks, tokens blockIdx.x, + gridDim.x, ...; thread i owns
+// chunk i of every branch, with its weights and its weight-gradient sums in registers.  The rows of a
+// token (d_state, d_normed, state, values; (3 HC + 1) * H * 2 bytes) arrive by bulk copies in one of
+// two stages while the token before is computed.  One reduction gives all sums over the rows, a second
+// one the mean that the norm behind the block needs.
+// Bound: HBM, (4 HC + 2) * H * 2 bytes a token.
+template <int HC>
 __global__ void __launch_bounds__(512) inject_norm_bwd_kernel(const InjectNormBwdParams p) {
+    extern __shared__ __align__(128) uint8_t stages[];
+    __shared__ float red[16][32], red1[16];
+    __shared__ uint64_t full[2];
+    const int nc = p.H / 8, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nw = blockDim.x >> 5;
+    const int rows = (p.d_state ? HC : 0) + (p.d_normed ? HC : 0) + HC + 1;
+    const uint32_t row_bytes = p.H * 2, stage_bytes = rows * row_bytes;
+    const bool mine = tid < nc;
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    if (tid == 0) {
+        mbar_init(&full[0], 1);
+        mbar_init(&full[1], 1);
+        fence_mbar_init();
+    }
+    __syncthreads();
+    // stage layout: state, values, d_state, d_normed
+    const int off_D = HC + 1, off_n = off_D + (p.d_state ? HC : 0);
+    auto fetch = [&](long long t, int s) {
+        const uint32_t b = smem_u32(stages + (size_t)s * stage_bytes);
+        mbar_arrive_expect_tx(&full[s], stage_bytes);
+        const uint64_t once = l2_evict_first();
+        bulk_load(b, p.state + t * HC * p.H, HC * row_bytes, &full[s], once);
+        bulk_load(b + HC * row_bytes, p.values + t * p.H, row_bytes, &full[s], once);
+        if (p.d_state) bulk_load(b + off_D * row_bytes, p.d_state + t * HC * p.H, HC * row_bytes, &full[s], once);
+        if (p.d_normed) bulk_load(b + off_n * row_bytes, p.d_normed + t * HC * p.H, HC * row_bytes, &full[s], once);
+    };
+    if (tid == 0)
+        for (int k = 0; k < 2; ++k)
+            if (blockIdx.x + (long long)k * gridDim.x < p.batch) fetch(blockIdx.x + (long long)k * gridDim.x, k);
+
+    uint4 wn[HC], wp = zero;
+    float an[HC][8], ap[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) ap[k] = 0.f;
+#pragma unroll
+    for (int b = 0; b < HC; ++b) {
+        wn[b] = mine && p.w_next ? reinterpret_cast<const uint4*>(p.w_next)[b * nc + tid] : zero;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) an[b][k] = 0.f;
+    }
+    if (mine && p.w_post) wp = reinterpret_cast<const uint4*>(p.w_post)[tid];
+
+    int it = 0;
+    for (long long t = blockIdx.x; t < p.batch; t += gridDim.x, ++it) {
+        const int st = it & 1;
+        if (!mbar_wait(&full[st], (it >> 1) & 1)) break;     // (every thread times out alike: the copy never came)
+        const uint4* S = reinterpret_cast<const uint4*>(stages + (size_t)st * stage_bytes);
+        const uint4 y4 = mine ? S[HC * nc + tid] : zero;
+        // per branch s^2, e s, D z0, e z0, s z0 (five each), and y^2 last; z0 = y (1 + wp)
+        float v[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = 0.f;
+        if (mine) {
+            float y[8], w[8], z0[8];
+            unpack8(y4, y);
+            unpack8(wp, w);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                z0[k] = y[k] * (1.0f + w[k]);
+                v[5 * HC] = fmaf(y[k], y[k], v[5 * HC]);
+            }
+#pragma unroll
+            for (int b = 0; b < HC; ++b) {
+                float s[8], x[8];
+                unpack8(S[b * nc + tid], s);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    v[5 * b] = fmaf(s[k], s[k], v[5 * b]);
+                    v[5 * b + 4] = fmaf(s[k], z0[k], v[5 * b + 4]);
+                }
+                if (p.d_state) {
+                    unpack8(S[(off_D + b) * nc + tid], x);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) v[5 * b + 2] = fmaf(x[k], z0[k], v[5 * b + 2]);
+                }
+                if (p.d_normed) {
+                    unpack8(S[(off_n + b) * nc + tid], x);
+                    unpack8(wn[b], w);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const float e = x[k] * (1.0f + w[k]);
+                        v[5 * b + 1] = fmaf(e, s[k], v[5 * b + 1]);
+                        v[5 * b + 3] = fmaf(e, z0[k], v[5 * b + 3]);
+                    }
+                }
+            }
+        }
+        red[warp][lane] = warp_sums32(v);
+        __syncthreads();
+        float tot = 0.f;                                     // value `lane`, over the block
+        for (int i = 0; i < nw; ++i) tot += red[i][lane];
+        // lane b: the scalars of branch b
+        const int lb = lane < HC ? lane : 0;
+        const float ss = __shfl_sync(0xffffffffu, tot, 5 * lb), es = __shfl_sync(0xffffffffu, tot, 5 * lb + 1);
+        const float dz_D = __shfl_sync(0xffffffffu, tot, 5 * lb + 2), dz_e = __shfl_sync(0xffffffffu, tot, 5 * lb + 3);
+        const float dz_s = __shfl_sync(0xffffffffu, tot, 5 * lb + 4), yy = __shfl_sync(0xffffffffu, tot, 5 * HC);
+        const float rv = p.w_post ? rms_scale(yy, p.H, p.eps) : 1.0f;
+        const float rs_l = rms_scale(ss, p.H, p.eps), m_l = es / (float)p.H * rs_l * rs_l;
+        const float g_l = (p.gate ? bf2f(p.gate[t * HC + lb]) : 1.0f) * p.scale;
+        if (tid < HC && p.d_gate) p.d_gate[t * HC + tid] = f2bf(p.scale * rv * (dz_D + rs_l * (dz_e - m_l * dz_s)));
+        float dz[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) dz[k] = 0.f;
+#pragma unroll
+        for (int b = 0; b < HC; ++b) {
+            const float rs = __shfl_sync(0xffffffffu, rs_l, b), m = __shfl_sync(0xffffffffu, m_l, b);
+            const float gb = __shfl_sync(0xffffffffu, g_l, b);
+            if (mine) {
+                float s[8], D[8], n[8], w[8];
+                unpack8(S[b * nc + tid], s);
+                unpack8(p.d_state ? S[(off_D + b) * nc + tid] : zero, D);
+                unpack8(p.d_normed ? S[(off_n + b) * nc + tid] : zero, n);
+                unpack8(wn[b], w);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    D[k] = fmaf(rs, n[k] * (1.0f + w[k]) - s[k] * m, D[k]);
+                    dz[k] = fmaf(gb, D[k], dz[k]);
+                    an[b][k] = fmaf(n[k] * rs, s[k], an[b][k]);
+                }
+                reinterpret_cast<uint4*>(p.d_hyper)[(t * HC + b) * nc + tid] = pack8(D);
+            }
+        }
+        float y[8], w[8], q = 0.f;
+        unpack8(y4, y);
+        unpack8(wp, w);
+        if (p.w_post) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) q = fmaf(dz[k] * (1.0f + w[k]), y[k], q);      // zero where !mine
+#pragma unroll
+            for (int o = 16; o; o >>= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
+            if (lane == 0) red1[warp] = q;
+        }
+        __syncthreads();                                     // the stage and `red` are read; red1 is written
+        if (tid == 0 && t + 2LL * gridDim.x < p.batch) fetch(t + 2LL * gridDim.x, st);
+        if (p.w_post) {
+            q = 0.f;
+            for (int i = 0; i < nw; ++i) q += red1[i];
+            const float mq = q / (float)p.H * rv * rv;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                ap[k] = fmaf(dz[k] * rv, y[k], ap[k]);
+                dz[k] = rv * (dz[k] * (1.0f + w[k]) - y[k] * mq);
+            }
+        }
+        if (mine) reinterpret_cast<uint4*>(p.d_values)[t * nc + tid] = pack8(dz);
+    }
+    if (mine) {
+        float4* out = reinterpret_cast<float4*>(p.part + (size_t)blockIdx.x * (HC + 1) * p.H) + 2 * tid;
+#pragma unroll
+        for (int b = 0; b < HC; ++b) {
+            out[(size_t)b * 2 * nc] = make_float4(an[b][0], an[b][1], an[b][2], an[b][3]);
+            out[(size_t)b * 2 * nc + 1] = make_float4(an[b][4], an[b][5], an[b][6], an[b][7]);
+        }
+        out[(size_t)HC * 2 * nc] = make_float4(ap[0], ap[1], ap[2], ap[3]);
+        out[(size_t)HC * 2 * nc + 1] = make_float4(ap[4], ap[5], ap[6], ap[7]);
+    }
+}
+
+// The backward for wider rows: every thread owns several chunks, whose weight-gradient sums it keeps in
+// shared memory over all of its block's tokens, and reads the rows twice.
+__global__ void __launch_bounds__(512) inject_norm_bwd_wide_kernel(const InjectNormBwdParams p) {
     extern __shared__ __align__(16) float acc[];           // [(HC + 1) * H], then dz [H]
     __shared__ float red[32 * 6];
     const int nc = p.H / 8;
