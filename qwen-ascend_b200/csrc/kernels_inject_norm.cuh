@@ -53,6 +53,48 @@ FNX_DEV void unpack8(const uint4& u, float (&f)[8]) {
 FNX_DEV uint4 pack8(const float (&f)[8]) {
     return make_uint4(pack_bf2(f[0], f[1]), pack_bf2(f[2], f[3]), pack_bf2(f[4], f[5]), pack_bf2(f[6], f[7]));
 }
+// Pairs of floats in one register pair: two fp32 operations per instruction, each rounded as the scalar
+// one.  A bf16 pair widens to one in two instructions.
+typedef unsigned long long f32x2;
+FNX_DEV f32x2 f2_make(float lo, float hi) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+FNX_DEV float2 f2_get(f32x2 a) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a));
+    return r;
+}
+FNX_DEV f32x2 f2_fma(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+FNX_DEV f32x2 f2_mul(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+FNX_DEV f32x2 f2_add(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+FNX_DEV float f2_sum(f32x2 a) {
+    const float2 v = f2_get(a);
+    return v.x + v.y;
+}
+FNX_DEV f32x2 f2_bf16(uint32_t u) { return f2_make(bf_lo(u), bf_hi(u)); }
+FNX_DEV void widen8(const uint4& u, f32x2 (&f)[4]) {
+    f[0] = f2_bf16(u.x); f[1] = f2_bf16(u.y); f[2] = f2_bf16(u.z); f[3] = f2_bf16(u.w);
+}
+FNX_DEV uint32_t f2_round(f32x2 a) {
+    const float2 v = f2_get(a);
+    return pack_bf2(v.x, v.y);
+}
+FNX_DEV uint4 round8(const f32x2 (&f)[4]) { return make_uint4(f2_round(f[0]), f2_round(f[1]), f2_round(f[2]), f2_round(f[3])); }
+
 FNX_DEV float rms_scale(float sum_sq, int H, float eps) {
     return __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(sum_sq, (float)H), eps)));
 }
@@ -211,15 +253,16 @@ __global__ void __launch_bounds__(512) inject_norm_bwd_kernel(const InjectNormBw
         for (int k = 0; k < 2; ++k)
             if (blockIdx.x + (long long)k * gridDim.x < p.batch) fetch(blockIdx.x + (long long)k * gridDim.x, k);
 
+    const f32x2 one2 = f2_make(1.f, 1.f), zero2 = f2_make(0.f, 0.f);
     uint4 wn[HC], wp = zero;
-    float an[HC][8], ap[8];
+    f32x2 an[HC][4], ap[4];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) ap[k] = 0.f;
+    for (int k = 0; k < 4; ++k) ap[k] = zero2;
 #pragma unroll
     for (int b = 0; b < HC; ++b) {
         wn[b] = mine && p.w_next ? reinterpret_cast<const uint4*>(p.w_next)[b * nc + tid] : zero;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) an[b][k] = 0.f;
+        for (int k = 0; k < 4; ++k) an[b][k] = zero2;
     }
     if (mine && p.w_post) wp = reinterpret_cast<const uint4*>(p.w_post)[tid];
 
@@ -234,37 +277,46 @@ __global__ void __launch_bounds__(512) inject_norm_bwd_kernel(const InjectNormBw
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = 0.f;
         if (mine) {
-            float y[8], w[8], z0[8];
-            unpack8(y4, y);
-            unpack8(wp, w);
+            f32x2 z0[4], x[4], w[4], q0 = zero2;
+            widen8(y4, x);
+            widen8(wp, w);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                z0[k] = y[k] * (1.0f + w[k]);
-                v[5 * HC] = fmaf(y[k], y[k], v[5 * HC]);
+            for (int k = 0; k < 4; ++k) {
+                z0[k] = f2_mul(x[k], f2_add(one2, w[k]));
+                q0 = f2_fma(x[k], x[k], q0);
             }
+            v[5 * HC] = f2_sum(q0);
 #pragma unroll
             for (int b = 0; b < HC; ++b) {
-                float s[8], x[8];
-                unpack8(S[b * nc + tid], s);
+                f32x2 s[4], q1 = zero2;
+                q0 = zero2;
+                widen8(S[b * nc + tid], s);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    v[5 * b] = fmaf(s[k], s[k], v[5 * b]);
-                    v[5 * b + 4] = fmaf(s[k], z0[k], v[5 * b + 4]);
+                for (int k = 0; k < 4; ++k) {
+                    q0 = f2_fma(s[k], s[k], q0);
+                    q1 = f2_fma(s[k], z0[k], q1);
                 }
+                v[5 * b] = f2_sum(q0);
+                v[5 * b + 4] = f2_sum(q1);
                 if (p.d_state) {
-                    unpack8(S[(off_D + b) * nc + tid], x);
+                    q0 = zero2;
+                    widen8(S[(off_D + b) * nc + tid], x);
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) v[5 * b + 2] = fmaf(x[k], z0[k], v[5 * b + 2]);
+                    for (int k = 0; k < 4; ++k) q0 = f2_fma(x[k], z0[k], q0);
+                    v[5 * b + 2] = f2_sum(q0);
                 }
                 if (p.d_normed) {
-                    unpack8(S[(off_n + b) * nc + tid], x);
-                    unpack8(wn[b], w);
+                    q0 = q1 = zero2;
+                    widen8(S[(off_n + b) * nc + tid], x);
+                    widen8(wn[b], w);
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const float e = x[k] * (1.0f + w[k]);
-                        v[5 * b + 1] = fmaf(e, s[k], v[5 * b + 1]);
-                        v[5 * b + 3] = fmaf(e, z0[k], v[5 * b + 3]);
+                    for (int k = 0; k < 4; ++k) {
+                        const f32x2 e = f2_mul(x[k], f2_add(one2, w[k]));
+                        q0 = f2_fma(e, s[k], q0);
+                        q1 = f2_fma(e, z0[k], q1);
                     }
+                    v[5 * b + 1] = f2_sum(q0);
+                    v[5 * b + 3] = f2_sum(q1);
                 }
             }
         }
@@ -281,34 +333,39 @@ __global__ void __launch_bounds__(512) inject_norm_bwd_kernel(const InjectNormBw
         const float rs_l = rms_scale(ss, p.H, p.eps), m_l = es / (float)p.H * rs_l * rs_l;
         const float g_l = (p.gate ? bf2f(p.gate[t * HC + lb]) : 1.0f) * p.scale;
         if (tid < HC && p.d_gate) p.d_gate[t * HC + tid] = f2bf(p.scale * rv * (dz_D + rs_l * (dz_e - m_l * dz_s)));
-        float dz[8];
+        f32x2 dz[4];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) dz[k] = 0.f;
+        for (int k = 0; k < 4; ++k) dz[k] = zero2;
 #pragma unroll
         for (int b = 0; b < HC; ++b) {
-            const float rs = __shfl_sync(0xffffffffu, rs_l, b), m = __shfl_sync(0xffffffffu, m_l, b);
-            const float gb = __shfl_sync(0xffffffffu, g_l, b);
+            const float rs1 = __shfl_sync(0xffffffffu, rs_l, b), m1 = -__shfl_sync(0xffffffffu, m_l, b);
+            const float g1 = __shfl_sync(0xffffffffu, g_l, b);
             if (mine) {
-                float s[8], D[8], n[8], w[8];
-                unpack8(S[b * nc + tid], s);
-                unpack8(p.d_state ? S[(off_D + b) * nc + tid] : zero, D);
-                unpack8(p.d_normed ? S[(off_n + b) * nc + tid] : zero, n);
-                unpack8(wn[b], w);
+                const f32x2 rs = f2_make(rs1, rs1), m = f2_make(m1, m1), gb = f2_make(g1, g1);
+                f32x2 s[4], D[4], n[4], w[4];
+                widen8(S[b * nc + tid], s);
+                widen8(p.d_state ? S[(off_D + b) * nc + tid] : zero, D);
+                widen8(p.d_normed ? S[(off_n + b) * nc + tid] : zero, n);
+                widen8(wn[b], w);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    D[k] = fmaf(rs, n[k] * (1.0f + w[k]) - s[k] * m, D[k]);
-                    dz[k] = fmaf(gb, D[k], dz[k]);
-                    an[b][k] = fmaf(n[k] * rs, s[k], an[b][k]);
+                for (int k = 0; k < 4; ++k) {
+                    const f32x2 e = f2_mul(n[k], f2_add(one2, w[k]));
+                    D[k] = f2_fma(rs, f2_fma(s[k], m, e), D[k]);
+                    dz[k] = f2_fma(gb, D[k], dz[k]);
+                    an[b][k] = f2_fma(f2_mul(n[k], rs), s[k], an[b][k]);
                 }
-                reinterpret_cast<uint4*>(p.d_hyper)[(t * HC + b) * nc + tid] = pack8(D);
+                reinterpret_cast<uint4*>(p.d_hyper)[(t * HC + b) * nc + tid] = round8(D);
             }
         }
-        float y[8], w[8], q = 0.f;
-        unpack8(y4, y);
-        unpack8(wp, w);
+        f32x2 y[4], w[4];
+        float q = 0.f;
+        widen8(y4, y);
+        widen8(wp, w);
         if (p.w_post) {
+            f32x2 q0 = zero2;                                // zero where !mine
 #pragma unroll
-            for (int k = 0; k < 8; ++k) q = fmaf(dz[k] * (1.0f + w[k]), y[k], q);      // zero where !mine
+            for (int k = 0; k < 4; ++k) q0 = f2_fma(f2_mul(dz[k], f2_add(one2, w[k])), y[k], q0);
+            q = f2_sum(q0);
 #pragma unroll
             for (int o = 16; o; o >>= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
             if (lane == 0) red1[warp] = q;
@@ -318,24 +375,28 @@ __global__ void __launch_bounds__(512) inject_norm_bwd_kernel(const InjectNormBw
         if (p.w_post) {
             q = 0.f;
             for (int i = 0; i < nw; ++i) q += red1[i];
-            const float mq = q / (float)p.H * rv * rv;
+            const float mq = -q / (float)p.H * rv * rv;
+            const f32x2 mq2 = f2_make(mq, mq), rv2 = f2_make(rv, rv);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                ap[k] = fmaf(dz[k] * rv, y[k], ap[k]);
-                dz[k] = rv * (dz[k] * (1.0f + w[k]) - y[k] * mq);
+            for (int k = 0; k < 4; ++k) {
+                ap[k] = f2_fma(f2_mul(dz[k], rv2), y[k], ap[k]);
+                dz[k] = f2_mul(rv2, f2_fma(y[k], mq2, f2_mul(dz[k], f2_add(one2, w[k]))));
             }
         }
-        if (mine) reinterpret_cast<uint4*>(p.d_values)[t * nc + tid] = pack8(dz);
+        if (mine) reinterpret_cast<uint4*>(p.d_values)[t * nc + tid] = round8(dz);
     }
     if (mine) {
         float4* out = reinterpret_cast<float4*>(p.part + (size_t)blockIdx.x * (HC + 1) * p.H) + 2 * tid;
+        auto put = [&](size_t at, const f32x2 (&a)[4]) {
 #pragma unroll
-        for (int b = 0; b < HC; ++b) {
-            out[(size_t)b * 2 * nc] = make_float4(an[b][0], an[b][1], an[b][2], an[b][3]);
-            out[(size_t)b * 2 * nc + 1] = make_float4(an[b][4], an[b][5], an[b][6], an[b][7]);
-        }
-        out[(size_t)HC * 2 * nc] = make_float4(ap[0], ap[1], ap[2], ap[3]);
-        out[(size_t)HC * 2 * nc + 1] = make_float4(ap[4], ap[5], ap[6], ap[7]);
+            for (int k = 0; k < 2; ++k) {
+                const float2 lo = f2_get(a[2 * k]), hi = f2_get(a[2 * k + 1]);
+                out[at + k] = make_float4(lo.x, lo.y, hi.x, hi.y);
+            }
+        };
+#pragma unroll
+        for (int b = 0; b < HC; ++b) put((size_t)b * 2 * nc, an[b]);
+        put((size_t)HC * 2 * nc, ap);
     }
 }
 
@@ -445,8 +506,10 @@ __global__ void __launch_bounds__(256) column_sum_kernel(const float* __restrict
     const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5;
     const int c = blockIdx.x * 32 + lane;
     float s = 0.f;
-    if (c < n)
+    if (c < n) {
+#pragma unroll 8
         for (int r = grp; r < rows; r += 8) s += part[(size_t)r * n + c];
+    }
     red[grp][lane] = s;
     __syncthreads();
     if (grp == 0 && c < n) {
