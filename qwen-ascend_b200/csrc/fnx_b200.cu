@@ -1440,6 +1440,54 @@ int w4_dense_launch_t(const W4DenseParams& p, int CL, cudaStream_t st) {
     if (cudaLaunchKernelEx(&cfg, w4_dense_kernel<WPL, NT>, p) != cudaSuccess) return FNX_ELAUNCH;
     return launch_rc();
 }
+
+template <int NT>
+int w4_dense_tma_launch_t(const W4DenseParams& d, int CL, cudaStream_t st) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return FNX_EDRIVER;
+    W4TmaParams p;
+    p.d = d;
+    p.gshift = -1;
+    p.stages = 0;
+    for (int b = 0; b < 20; ++b)
+        if (d.gs == 16 << b) p.gshift = b;
+    p.srows = d.gs % W4T_ROWS == 0 ? 1 : W4T_ROWS % d.gs == 0 ? W4T_ROWS / d.gs : (W4T_ROWS - 1) / d.gs + 2;
+    p.stages = w4_tma_stages(NT, p.srows);
+    auto map = [&](CUtensorMap* m, CUtensorMapDataType dt, const void* ptr, unsigned long long cols, unsigned long long rows,
+                   unsigned long long pitch, unsigned b0, unsigned b1, CUtensorMapSwizzle swz) {
+        const cuuint64_t dims[2] = {cols, rows}, strides[1] = {pitch};
+        const cuuint32_t box[2] = {b0, b1}, one[2] = {1, 1};
+        return fn(m, dt, 2, const_cast<void*>(ptr), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    };
+    if (!map(&p.tw, CU_TENSOR_MAP_DATA_TYPE_INT32, d.w, d.N / 8, d.K, d.N / 2, 32, W4T_ROWS, CU_TENSOR_MAP_SWIZZLE_128B) ||
+        !map(&p.tx, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, d.x, d.K, d.M, d.ld_x * 2, 64, 8 * NT, CU_TENSOR_MAP_SWIZZLE_128B) ||
+        !map(&p.ts, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, d.s, d.N, (d.K + d.gs - 1) / d.gs, d.N * 2ull, W4D_FEATS, p.srows,
+             CU_TENSOR_MAP_SWIZZLE_NONE))
+        return FNX_EALIGN;
+    static bool configured[FNX_MAX_DEVICES] = {};
+    const int dev = current_device();
+    if (!configured[dev]) {
+        if (cudaFuncSetAttribute(w4_dense_tma_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 113 * 1024) != cudaSuccess)   // every ring and sum (w4_tma_stages)
+            return FNX_ELAUNCH;
+        configured[dev] = true;
+    }
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1;
+    attr[0].val.clusterDim.y = (unsigned)CL;
+    attr[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((d.N + W4D_FEATS - 1) / W4D_FEATS), (unsigned)CL, (unsigned)((d.M + 8 * NT - 1) / (8 * NT)));
+    cfg.blockDim = dim3(W4D_THREADS, 1, 1);
+    cfg.dynamicSmemBytes = w4_dense_tma_smem<NT>(d.M, p.srows);
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, w4_dense_tma_kernel<NT>, p) != cudaSuccess) return FNX_ELAUNCH;
+    return launch_rc();
+}
 }  // namespace
 
 FNX_API int fnx_w4a16_gemv(const void* x, long long ld_x, const void* w4, const void* scales, void* y, int M, int K,
@@ -1455,6 +1503,21 @@ FNX_API int fnx_w4a16_gemv(const void* x, long long ld_x, const void* w4, const 
     int CL = 1;
     while (CL < 8 && tiles * CL < 2 * num_sms() && K / (16 * CL) >= 16) CL *= 2;
     cudaStream_t st = (cudaStream_t)stream;
+    static const int tma = env_int("FNX_W4_TMA", -1), cl = env_int("FNX_W4_CL", 0);
+    if (N % 32 == 0 && ld_x % 8 == 0 && (tma < 0 ? (long long)K * N >= 16 << 20 : tma)) {
+        // parts of K: the SM with the most CTAs works through its stages one after another, and every
+        // part costs a start and the cluster's sum (about three stages)
+        const int stages = (K + W4T_ROWS - 1) / W4T_ROWS;
+        int C = 1;
+        long long best = 1LL << 60;
+        for (int c = 1; c <= 8 && c <= stages; ++c) {
+            const long long per_sm = (tiles * c + num_sms() - 1) / num_sms();
+            const long long cost = per_sm * ((stages + c - 1) / c) + 3 * ((per_sm + 1) / 2) + (per_sm == 1 ? (stages + c - 1) / c / 2 : 0);
+            if (cost < best) best = cost, C = c;
+        }
+        if (cl) C = cl;
+        return NT == 2 ? w4_dense_tma_launch_t<2>(p, C, st) : w4_dense_tma_launch_t<1>(p, C, st);
+    }
     if (NT == 2) return w4_dense_launch_t<1, 2>(p, CL, st);
     if (N % 16 == 0) return w4_dense_launch_t<2, 1>(p, CL, st);
     return w4_dense_launch_t<1, 1>(p, CL, st);
