@@ -57,6 +57,24 @@ inline int launch_rc() {
     return e == cudaSuccess ? FNX_OK : FNX_ELAUNCH;
 }
 
+// Launch as a programmatic dependent of the kernel before it on the stream: the kernel starts while that
+// one ends and has to wait for it (pdl_wait) before it reads or writes global memory.
+template <typename... Params, typename... Args>
+inline int launch_pdl(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t st, Args&&... args) {
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...) != cudaSuccess) return FNX_ELAUNCH;
+    return launch_rc();
+}
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 inline int grid_for(long long work, int threads) {
@@ -277,11 +295,6 @@ int gemm_check(int mode, int epi, const GemmParams& p) {
     return FNX_OK;
 }
 
-int env_int(const char* name, int dflt) {
-    const char* e = getenv(name);
-    return e && *e ? atoi(e) : dflt;
-}
-
 size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 
 }  // namespace
@@ -406,8 +419,7 @@ bool inject_norm_shape(int batch, int H, int HC) {
 template <int NV, int BR>
 int inject_norm_launch_t(const InjectNormParams& p, int batch, cudaStream_t st) {
     const int threads = ((p.H / 8 + NV - 1) / NV + 31) / 32 * 32;
-    inject_norm_kernel<NV, BR><<<dim3((unsigned)batch, (unsigned)((p.HC + BR - 1) / BR)), threads, 0, st>>>(p);
-    return launch_rc();
+    return launch_pdl(inject_norm_kernel<NV, BR>, dim3((unsigned)batch, (unsigned)((p.HC + BR - 1) / BR)), threads, 0, st, p);
 }
 
 template <int BR>
@@ -441,8 +453,8 @@ int inject_norm_bwd_launch(const InjectNormBwdParams& p, int blocks, cudaStream_
             return FNX_ELAUNCH;
         configured[dev] = true;
     }
-    inject_norm_bwd_kernel<HC><<<blocks, (p.H / 8 + 31) / 32 * 32, inject_norm_bwd_smem(p.H, HC), st>>>(p);
-    return launch_rc();
+    return launch_pdl(inject_norm_bwd_kernel<HC>, dim3((unsigned)blocks), (p.H / 8 + 31) / 32 * 32,
+                      inject_norm_bwd_smem(p.H, HC), st, p);
 }
 }  // namespace
 
@@ -502,16 +514,14 @@ FNX_API int fnx_inject_norm_backward(const void* d_state, const void* d_normed, 
                     return FNX_ELAUNCH;
                 configured[dev] = true;
             }
-            inject_norm_bwd_wide_kernel<<<blocks, 512, inject_norm_bwd_smem(H, HC), st>>>(p);
-            rc = launch_rc();
+            rc = launch_pdl(inject_norm_bwd_wide_kernel, dim3((unsigned)blocks), 512, inject_norm_bwd_smem(H, HC), st, p);
         }
         if (rc) return rc;
     }
     if (d_w_next || d_w_post) {
         const int n = (HC + 1) * H;
-        column_sum_kernel<<<(n + 31) / 32, 256, 0, st>>>((const float*)ws, (bf16*)d_w_next, (bf16*)d_w_post, blocks,
-                                                         HC * H, n);
-        return launch_rc();
+        return launch_pdl(column_sum_kernel, dim3((unsigned)((n + 31) / 32)), 256, 0, st, (const float*)ws, (bf16*)d_w_next,
+                          (bf16*)d_w_post, blocks, HC * H, n);
     }
     return FNX_OK;
 }
@@ -1219,7 +1229,7 @@ int ffn_pair_width(const FfnGemm& g, int epi, int pairs) {
 }
 
 template <int EPI>
-int ffn_pair_launch(const FfnGemm* g, int count, float* gu, bool chained, cudaStream_t st) {
+int ffn_pair_launch(const FfnGemm* g, int count, float* gu, bool followed, cudaStream_t st) {
     const size_t smem = ffn_gemm_smem(EPI);
     static bool configured[FNX_MAX_DEVICES] = {};
     const int dev = current_device();
@@ -1232,11 +1242,10 @@ int ffn_pair_launch(const FfnGemm* g, int count, float* gu, bool chained, cudaSt
     FfnParams p;
     memset(&p, 0, sizeof p);
     const int pairs = num_sms() / 2;
-    static const int bn_env = env_int("FNX_FFN_PAIR_BN", 0);
     long long total = 0;
     for (int i = 0; i < count; ++i) {
         FfnProduct& q = p.q[i];
-        q.bn = bn_env && !g[i].bmn ? bn_env : count > 1 ? 256 : ffn_pair_width(g[i], EPI, pairs);
+        q.bn = count > 1 ? 256 : ffn_pair_width(g[i], EPI, pairs);
         int rc = ffn_maps(g[i], EPI, &q.ta, &q.tb, 128, q.bn / 2);
         if (!rc) rc = ffn_map(&q.tc, g[i].c, g[i].N, g[i].M, g[i].ldc, 64, 32);
         if (!rc && EPI == FF_DGATE)
@@ -1250,7 +1259,7 @@ int ffn_pair_launch(const FfnGemm* g, int count, float* gu, bool chained, cudaSt
         total += (long long)q.mt * q.nt;
     }
     if (total > 0x3fffffffLL) return FNX_ESHAPE;
-    p.gu = gu; p.count = count; p.total = (int)total;
+    p.gu = gu; p.count = count; p.total = (int)total; p.followed = followed;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 2;
@@ -1264,14 +1273,14 @@ int ffn_pair_launch(const FfnGemm* g, int count, float* gu, bool chained, cudaSt
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cfg.attrs = attr;
-    cfg.numAttrs = chained ? 2 : 1;
+    cfg.numAttrs = 2;
     if (cudaLaunchKernelEx(&cfg, ffn_gemm_kernel<EPI>, p) != cudaSuccess) return FNX_ELAUNCH;
     return launch_rc();
 }
 
 template <int EPI, int BN>
 int ffn_small_launch(const FfnGemm* g, int count, float* gu, int CL, int a_rows, int stages, bool chained,
-                     cudaStream_t st) {
+                     bool followed, cudaStream_t st) {
     static bool configured[FNX_MAX_DEVICES] = {};
     const int dev = current_device();
     if (!configured[dev]) {
@@ -1296,6 +1305,7 @@ int ffn_small_launch(const FfnGemm* g, int count, float* gu, int CL, int a_rows,
         total += q.tiles;
     }
     p.gu = gu; p.count = count; p.a_rows = a_rows; p.stages = stages; p.CL = CL;
+    p.followed = followed;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = (unsigned)CL;
@@ -1309,15 +1319,17 @@ int ffn_small_launch(const FfnGemm* g, int count, float* gu, int CL, int a_rows,
     cfg.dynamicSmemBytes = 1024 + ffn_small_body(BN, a_rows, stages) + sizeof(FfnSmallSmem);
     cfg.stream = st;
     cfg.attrs = attr;
-    cfg.numAttrs = chained ? 2 : 1;
+    cfg.numAttrs = 2;
     if (cudaLaunchKernelEx(&cfg, ffn_small_kernel<EPI, BN>, p) != cudaSuccess) return FNX_ELAUNCH;
     return launch_rc();
 }
 
-// `count` products (more than one: FF_PLAIN) in one launch.  chained: it follows another launch of the
-// block on the stream, which writes none of the b operands.
+// `count` products (more than one: FF_PLAIN) in one launch, a programmatic dependent of the kernel before
+// it on the stream: it starts while that one ends and waits for it before it touches its data.
+// chained: that kernel is another launch of the block, which writes none of the b operands, so these
+// are fetched before the wait.  followed: so does the next one behind this launch.
 template <int EPI>
-int ffn_products(const FfnGemm* g, int count, float* gu, bool chained, cudaStream_t st) {
+int ffn_products(const FfnGemm* g, int count, float* gu, bool chained, bool followed, cudaStream_t st) {
     const int width = EPI == FF_GATED ? 2 : 1;
     long long t64 = 0, t128 = 0;
     int KB = 1 << 30, box_rows = 0, rows = 0;
@@ -1333,9 +1345,8 @@ int ffn_products(const FfnGemm* g, int count, float* gu, bool chained, cudaStrea
     }
     // Few rows: the weights' bytes are the work, 128-row tiles of them.  More rows: 64 columns, while
     // the tiles fit the SMs twice; beyond that CTA pairs, unless their 256 rows would be half empty.
-    static const int t64_env = env_int("FNX_FFN_T64", 256);
-    const bool few = rows <= 32, fits = t64 <= t64_env;
-    if (!few && !fits && rows > 128) return ffn_pair_launch<EPI>(g, count, gu, chained, st);
+    const bool few = rows <= 32, fits = t64 <= 256;
+    if (!few && !fits && rows > 128) return ffn_pair_launch<EPI>(g, count, gu, followed, st);
     const int BN = few || !fits ? 128 : 64;
     const long long tiles = BN == 64 ? t64 : t128;
     if (tiles > 0x7ffffffLL) return FNX_ESHAPE;
@@ -1347,8 +1358,8 @@ int ffn_products(const FfnGemm* g, int count, float* gu, bool chained, cudaStrea
     while (a_rows > 16 && a_rows / 2 >= box_rows) a_rows /= 2;
     int stages = 92 * 1024 / ((a_rows + BN) * 128);          // a ring that leaves room for a second CTA on the SM
     if (stages > FS_MAX_STAGES) stages = FS_MAX_STAGES;
-    if (BN == 64) return ffn_small_launch<EPI, 64>(g, count, gu, CL, a_rows, stages, chained, st);
-    return ffn_small_launch<EPI, 128>(g, count, gu, CL, a_rows, stages, chained, st);
+    if (BN == 64) return ffn_small_launch<EPI, 64>(g, count, gu, CL, a_rows, stages, chained, followed, st);
+    return ffn_small_launch<EPI, 128>(g, count, gu, CL, a_rows, stages, chained, followed, st);
 }
 
 int ffn_check(int M, int H, int I, int O) {
@@ -1374,10 +1385,10 @@ FNX_API int fnx_gated_ffn(const void* x, long long ld_x, const void* w_gu, const
     if (ld_x % 8) return FNX_EALIGN;
     cudaStream_t st = (cudaStream_t)stream;
     const FfnGemm gu{x, w_gu, h, nullptr, ld_x, H, I, M, I, H, 0, 0};
-    rc = ffn_products<FF_GATED>(&gu, 1, (float*)saved, false, st);
+    rc = ffn_products<FF_GATED>(&gu, 1, (float*)saved, false, y != nullptr, st);
     if (rc || !y) return rc;
     const FfnGemm down{h, w_down, y, nullptr, I, I, O, M, O, I, 0, 0};
-    return ffn_products<FF_PLAIN>(&down, 1, nullptr, true, st);
+    return ffn_products<FF_PLAIN>(&down, 1, nullptr, true, false, st);
 }
 
 FNX_API int fnx_gated_ffn_backward(const void* dy, long long ld_dy, const void* x, long long ld_x, const void* w_gu,
@@ -1399,7 +1410,7 @@ FNX_API int fnx_gated_ffn_backward(const void* dy, long long ld_dy, const void* 
         if (!aligned16(q)) return FNX_EALIGN;
     if (ld_dy % 8 || ld_x % 8) return FNX_EALIGN;
     const FfnGemm dh{dy, w_down, dgu, (bf16*)dgu + I, ld_dy, I, 2LL * I, M, I, O, 0, 1};
-    rc = ffn_products<FF_DGATE>(&dh, 1, (float*)const_cast<void*>(saved), false, st);
+    rc = ffn_products<FF_DGATE>(&dh, 1, (float*)const_cast<void*>(saved), false, dx || dw_gu || dw_down, st);
     if (rc) return rc;
     // the three products that follow, in one launch, the one with the longest tiles first
     FfnGemm g[FF_MAX_PRODUCTS];
@@ -1407,9 +1418,7 @@ FNX_API int fnx_gated_ffn_backward(const void* dy, long long ld_dy, const void* 
     if (dx) g[n++] = FfnGemm{dgu, w_gu, dx, nullptr, 2LL * I, H, H, M, H, 2 * I, 0, 1};
     if (dw_gu) g[n++] = FfnGemm{dgu, x, dw_gu, nullptr, 2LL * I, ld_x, H, 2 * I, H, M, 1, 1};
     if (dw_down) g[n++] = FfnGemm{dy, h, dw_down, nullptr, ld_dy, I, I, O, I, M, 1, 1};
-    static const int grp = env_int("FNX_FFN_GROUP", 1);
-    if (!grp) { for (int i = 0; i < n && !rc; ++i) rc = ffn_products<FF_PLAIN>(g + i, 1, nullptr, true, st); return rc; }
-    if (n) rc = ffn_products<FF_PLAIN>(g, n, nullptr, true, st);
+    if (n) rc = ffn_products<FF_PLAIN>(g, n, nullptr, true, false, st);
     return rc;
 }
 
@@ -1425,18 +1434,20 @@ int w4_dense_launch_t(const W4DenseParams& p, int CL, cudaStream_t st) {
             return FNX_ELAUNCH;
         configured[dev] = true;
     }
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 1;
     attr[0].val.clusterDim.y = (unsigned)CL;
     attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)((p.N + W4D_FEATS - 1) / W4D_FEATS), (unsigned)CL, (unsigned)((p.M + 8 * NT - 1) / (8 * NT)));
     cfg.blockDim = dim3(W4D_THREADS, 1, 1);
     cfg.dynamicSmemBytes = w4_dense_smem<WPL, NT>(p.M);
     cfg.stream = st;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     if (cudaLaunchKernelEx(&cfg, w4_dense_kernel<WPL, NT>, p) != cudaSuccess) return FNX_ELAUNCH;
     return launch_rc();
 }
@@ -1473,18 +1484,20 @@ int w4_dense_tma_launch_t(const W4DenseParams& d, int CL, cudaStream_t st) {
             return FNX_ELAUNCH;
         configured[dev] = true;
     }
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 1;
     attr[0].val.clusterDim.y = (unsigned)CL;
     attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)((d.N + W4D_FEATS - 1) / W4D_FEATS), (unsigned)CL, (unsigned)((d.M + 8 * NT - 1) / (8 * NT)));
     cfg.blockDim = dim3(W4D_THREADS, 1, 1);
     cfg.dynamicSmemBytes = w4_dense_tma_smem<NT>(d.M, p.srows);
     cfg.stream = st;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     if (cudaLaunchKernelEx(&cfg, w4_dense_tma_kernel<NT>, p) != cudaSuccess) return FNX_ELAUNCH;
     return launch_rc();
 }
@@ -1503,8 +1516,9 @@ FNX_API int fnx_w4a16_gemv(const void* x, long long ld_x, const void* w4, const 
     int CL = 1;
     while (CL < 8 && tiles * CL < 2 * num_sms() && K / (16 * CL) >= 16) CL *= 2;
     cudaStream_t st = (cudaStream_t)stream;
-    static const int tma = env_int("FNX_W4_TMA", -1), cl = env_int("FNX_W4_CL", 0);
-    if (N % 32 == 0 && ld_x % 8 == 0 && (tma < 0 ? (long long)K * N >= 16 << 20 : tma)) {
+    // from 8 MB of weights on the ring of TMA copies (2048 x 16384, 8 tokens: 10.0 us against 15.6); below,
+    // the two are within 0.3 us of each other and the direct loads need no tensor maps (1.4 us of host time)
+    if (N % 32 == 0 && ld_x % 8 == 0 && (long long)K * N >= 16 << 20) {
         // parts of K: the SM with the most CTAs works through its stages one after another, and every
         // part costs a start and the cluster's sum (about three stages)
         const int stages = (K + W4T_ROWS - 1) / W4T_ROWS;
@@ -1515,7 +1529,6 @@ FNX_API int fnx_w4a16_gemv(const void* x, long long ld_x, const void* w4, const 
             const long long cost = per_sm * ((stages + c - 1) / c) + 3 * ((per_sm + 1) / 2) + (per_sm == 1 ? (stages + c - 1) / c / 2 : 0);
             if (cost < best) best = cost, C = c;
         }
-        if (cl) C = cl;
         return NT == 2 ? w4_dense_tma_launch_t<2>(p, C, st) : w4_dense_tma_launch_t<1>(p, C, st);
     }
     if (NT == 2) return w4_dense_launch_t<1, 2>(p, CL, st);
@@ -1567,6 +1580,11 @@ bool decode_v1() {
         v = (e && e[0] == '1') ? 1 : 0;
     }
     return v == 1;
+}
+
+int env_int(const char* name, int dflt) {
+    const char* e = getenv(name);
+    return e && *e ? atoi(e) : dflt;
 }
 
 

@@ -54,6 +54,7 @@ struct FfnParams {
     FfnProduct q[FF_MAX_PRODUCTS];
     float* gu;                       // g and u, blocked (see ffn_gu_index); NULL: not kept
     int count, total;
+    int followed;                    // another product of the chain follows: let it start at once
 };
 
 struct FfnSmem {
@@ -255,8 +256,10 @@ __global__ void __launch_bounds__(FF_THREADS, 1) ffn_gemm_kernel(const __grid_co
     cluster_sync_all();
     tc_fence_after();
     const uint32_t tmem = S.tmem_base;
-    pdl_launch_dependents();
-    pdl_wait();                                              // what the product before wrote or still reads
+    pdl_wait();                                              // what the kernel before wrote or still reads
+    // only now: the successor reads its weights before its own wait, which is safe once every CTA here
+    // has seen the kernels before this one complete
+    if (p.followed) pdl_launch_dependents();
 
     if (warp == 0) {
         // ------------------------------------------------ TMA copies of this CTA's halves
@@ -437,6 +440,7 @@ __global__ void __launch_bounds__(FF_THREADS, 1) ffn_gemm_kernel(const __grid_co
     // after a wait that expired: time for the copies and products in flight to end
     if (S.abort)
         for (int i = 0; i < 200; ++i) __nanosleep(1000);
+    if (!p.followed) pdl_launch_dependents();
     tc_fence_before();
     __syncthreads();
     cluster_sync_all();

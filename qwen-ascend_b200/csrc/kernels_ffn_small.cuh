@@ -8,8 +8,10 @@
 // copies as deep as shared memory allows); at more rows the latency of the chain of copies, products
 // and the cluster's sum.  Rows of A that do not exist are not loaded: the box holds p.a_rows (a power
 // of two >= M) and the tensor core multiplies whatever lies behind it into rows that are not stored.
-// A launch is a programmatic dependent of the product before it on the stream: its weights (operands
-// that no kernel of the chain writes, p.b_early) stream in while that one finishes, the rest waits.
+// A launch is a programmatic dependent of the kernel before it on the stream.  Behind another product
+// of the chain its weights (operands that no kernel of the chain writes, b_early) stream in while that
+// one finishes, the rest waits.  The last product of a chain lets its successor start when its own
+// products are done (9.9 against 10.3 us for one token when it did so at once).
 #pragma once
 #include <type_traits>
 
@@ -32,6 +34,7 @@ struct FfnSmallParams {
     FfnSmallProduct q[FF_MAX_PRODUCTS];
     float* gu;
     int count, a_rows, stages, CL;   // a_rows: rows of a K-major A's box
+    int followed;                    // another product of the chain follows: let it start at once
 };
 
 struct FfnSmallSmem {
@@ -94,7 +97,6 @@ __global__ void __launch_bounds__(FS_THREADS) ffn_small_kernel(const __grid_cons
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = S.tmem_base;
-    pdl_launch_dependents();
 
     if (warp == 0) {
         // ------------------------------------------------ TMA copies (a whole warp electing the issuer)
@@ -121,6 +123,9 @@ __global__ void __launch_bounds__(FS_THREADS) ffn_small_kernel(const __grid_cons
             }
         };
         if (!q.b_early) pdl_wait();
+        // a successor of the chain reads its weights before its own wait: it may start once every CTA
+        // here has seen the kernels before this one complete (followed only without b_early)
+        if (p.followed) pdl_launch_dependents();
         const int first = min(nkb, p.stages);
         if (elect_one())
             for (int j = 0; j < first; ++j) {
@@ -199,6 +204,7 @@ __global__ void __launch_bounds__(FS_THREADS) ffn_small_kernel(const __grid_cons
     __syncthreads();
     if (CL > 1) cluster_sync_all();
     pdl_wait();
+    if (!p.followed) pdl_launch_dependents();
 
     // ---------------------------------------------------- the ranks' shares of the tile
     constexpr int C4 = COLS / 4;

@@ -116,6 +116,7 @@ __global__ void __launch_bounds__(512) inject_norm_kernel(const InjectNormParams
     const int b0 = blockIdx.y * BR;
     const uint4* yv = reinterpret_cast<const uint4*>(p.values) + t * nc;
     const uint4* hv = reinterpret_cast<const uint4*>(p.hyper) + (t * p.HC + b0) * nc;
+    pdl_wait();
 
     uint4 y4[NV], h4[NV][BR];
 #pragma unroll
@@ -238,6 +239,8 @@ __global__ void __launch_bounds__(512) inject_norm_bwd_kernel(const InjectNormBw
         fence_mbar_init();
     }
     __syncthreads();
+    pdl_wait();
+    pdl_launch_dependents();
     // stage layout: state, values, d_state, d_normed
     const int off_D = HC + 1, off_n = off_D + (p.d_state ? HC : 0);
     auto fetch = [&](long long t, int s) {
@@ -408,6 +411,8 @@ __global__ void __launch_bounds__(512) inject_norm_bwd_wide_kernel(const InjectN
     const int nc = p.H / 8;
     float* dzs = acc + (size_t)(p.HC + 1) * p.H;
     for (int i = threadIdx.x; i < (p.HC + 1) * p.H; i += blockDim.x) acc[i] = 0.f;
+    pdl_wait();
+    pdl_launch_dependents();
     __syncthreads();
     const uint4 zero = make_uint4(0, 0, 0, 0);
     for (long long t = blockIdx.x; t < p.batch; t += gridDim.x) {
@@ -503,6 +508,8 @@ __global__ void __launch_bounds__(512) inject_norm_bwd_wide_kernel(const InjectN
 __global__ void __launch_bounds__(256) column_sum_kernel(const float* __restrict__ part, bf16* __restrict__ out0,
                                                          bf16* __restrict__ out1, int rows, int n0, int n) {
     __shared__ float red[8][33];
+    pdl_wait();
+    pdl_launch_dependents();
     const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5;
     const int c = blockIdx.x * 32 + lane;
     float s = 0.f;

@@ -71,6 +71,7 @@ template <int WPL, int NT>
 FNX_DEV void w4_dense_finish(const W4DenseParams& p, const float (&tot)[WPL][4][NT][4], float* red, int wn, int wk, int g,
                              int t, uint32_t rank, int CL, int m0, int mt) {
     constexpr int WF = 64 * WPL, WK = 8 / (W4D_FEATS / WF);
+    pdl_launch_dependents();
     const bool computes = wk < WK;              // (a copy warp takes part in the barriers and the sums)
     if (computes)
 #pragma unroll
@@ -146,6 +147,7 @@ __global__ void __launch_bounds__(W4D_THREADS, 2) w4_dense_kernel(const W4DenseP
     const bool col_ok = wc < words;
     const uint32_t* wp = p.w + wc;
 
+    pdl_wait();
     float tot[WPL][4][NT][4], acc[WPL][4][NT][4];
 #pragma unroll
     for (int a = 0; a < WPL; ++a)
@@ -299,6 +301,7 @@ __global__ void __launch_bounds__(W4D_THREADS, 2) w4_dense_tma_kernel(const __gr
         fence_mbar_init();
     }
     __syncthreads();
+    pdl_wait();
     const int NS = q.stages;
     auto fetch = [&](int j, int s) {                     // stage j of this CTA into slot s, by one thread
         const int row = (s0 + j) * W4T_ROWS;

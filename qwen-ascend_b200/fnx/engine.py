@@ -404,7 +404,6 @@ class DenseW4:
         if (self.w4.data_ptr() | self.sc.data_ptr()) % 16:
             raise ValueError("DenseW4: weights and scales must be 16-byte aligned")
         self._fn = _lib.lib().fnx_w4a16_gemv
-        self._pw, self._ps = self.w4.data_ptr(), self.sc.data_ptr()
 
     def __call__(self, x):
         shape, dev, K = x.shape, self.w4.device, self.K
@@ -423,7 +422,8 @@ class DenseW4:
         if one != 1 or ld % 4 or ld < K or x2.data_ptr() % 16:
             x2, ld = x2.clone(memory_format=torch.contiguous_format), K
         y = torch.empty(M, self.N, dtype=BF16, device=dev)
-        rc = self._fn(x2.data_ptr(), ld, self._pw, self._ps, y.data_ptr(), M, K, self.N, self.gs, _lib.raw_stream(dev))
+        rc = self._fn(x2.data_ptr(), ld, self.w4.data_ptr(), self.sc.data_ptr(), y.data_ptr(), M, K, self.N, self.gs,
+                      _lib.raw_stream(dev))
         _lib.check(rc, "W4A16 GEMV")
         return y if len(shape) == 2 else y.view(*shape[:-1], self.N)
 

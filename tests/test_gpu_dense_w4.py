@@ -49,7 +49,9 @@ def test_matches_the_definition(M, K, N, gs):
     check(lay, w, s, gs, torch.randn(M, K, generator=g).to(BF16).to(DEV))
 
 
-@pytest.mark.parametrize("M,K,N,gs", [(1, 8192, 28672, 128), (16, 4096, 14336, 32), (3, 2560, 151936, 64)])
+# from 2^24 weights on they come through the ring of copies: ragged K and N, groups that end inside a stage
+@pytest.mark.parametrize("M,K,N,gs", [(9, 5000, 4128, 48), (1, 4104, 4128, 16), (5, 8200, 2080, 4096), (17, 4096, 4104, 32),
+                                      (1, 8192, 28672, 128), (16, 4096, 14336, 32), (3, 2560, 151936, 64)])
 def test_wide(M, K, N, gs):
     lay, w, s = layer(K, N, gs)
     check(lay, w, s, gs, torch.randn(M, K, generator=torch.Generator().manual_seed(M)).to(BF16).to(DEV))
@@ -116,6 +118,23 @@ def test_rows_do_not_depend_on_their_batch_and_replay():
         z = lay(x)
     side.synchronize()
     assert torch.equal(z, held)
+
+
+@pytest.mark.parametrize("K,N", [(512, 256), (4096, 8192)])
+def test_inputs_written_just_before_and_just_after_a_call(K, N):
+    """A call may start while the kernel before it ends: it must see what that one writes, and the one
+    behind it must not overwrite what it still reads."""
+    lay, w, s = layer(K, N, 64)
+    a, b = (torch.randn(4, K, generator=torch.Generator().manual_seed(i)).to(BF16).to(DEV) for i in (1, 2))
+    ya, yb = lay(a), lay(b)
+    x = torch.empty_like(a)
+    outs = []
+    for i in range(40):
+        x.copy_(a if i % 2 else b)
+        outs.append(lay(x))
+        x.fill_(float("nan"))
+    for i, y in enumerate(outs):
+        assert torch.equal(y, ya if i % 2 else yb)
 
 
 def test_agrees_with_the_expert_gemm():

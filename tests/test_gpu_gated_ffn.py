@@ -75,7 +75,8 @@ def test_backward(M, H, I, O):
         close(got, want[name], name)
 
 
-@pytest.mark.parametrize("M,H,I", [(4096, 2560, 640), (2047, 4096, 4104)])
+# tiles of 160 and 192 columns, a last tile of few rows and few columns, all on CTA pairs
+@pytest.mark.parametrize("M,H,I", [(4096, 2560, 640), (2047, 4096, 4104), (3000, 1032, 1096), (1153, 2568, 1288)])
 def test_large(M, H, I):
     f, x, dy = make(M, H, I, H, 2)
     y, saved = f.forward_train(x)
@@ -190,6 +191,36 @@ def test_deterministic_on_other_streams_and_in_graphs():
     graph.replay()
     for a, b in zip(held, step()):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("M,H,I", [(1, 512, 256), (40, 1024, 512), (300, 512, 256), (2048, 1024, 1024)])
+def test_inputs_and_weights_written_just_before_and_just_after_a_call(M, H, I):
+    """Launches overlap the ends of the kernels before them: a step must see weights and rows that the
+    kernel just before it wrote, and the kernel behind it must not overwrite what it still reads."""
+    from fnx.gated_ffn import GatedFFN
+    two = [make(M, H, I, H, 8 + i) for i in range(2)]
+
+    def step(f, x, dy):
+        y, saved = f.forward_train(x)
+        return (y, f(x)) + f.backward(dy, saved)
+    want = [step(*t) for t in two]
+    f = GatedFFN(torch.empty_like(two[0][0].w_gu), torch.empty_like(two[0][0].w_down))
+    x, dy = torch.empty_like(two[0][1]), torch.empty_like(two[0][2])
+    for i in range(12):
+        src = two[i % 2]
+        for dst, s in ((x, src[1]), (dy, src[2]), (f.w_gu, src[0].w_gu), (f.w_down, src[0].w_down)):
+            dst.copy_(s)
+        got = step(f, x, dy)
+        for dst in (f.w_down, f.w_gu, x, dy):
+            dst.fill_(float("nan"))
+        for a, b in zip(got, want[i % 2]):
+            assert torch.equal(a, b)
+    f.w_gu.copy_(two[0][0].w_gu)
+    for i in range(12):                               # the down weights last, right before a forward
+        f.w_down.copy_(two[0][0].w_down)
+        y = f(two[0][1])
+        f.w_down.fill_(float("nan"))
+        assert torch.equal(y, want[0][1])
 
 
 def test_no_device_error_was_recorded():
