@@ -72,8 +72,6 @@ FNX_DEV void w4_dense_finish(const W4DenseParams& p, const float (&tot)[WPL][4][
                              int t, uint32_t rank, int CL, int m0, int mt) {
     constexpr int WF = 64 * WPL, WK = 8 / (W4D_FEATS / WF);
     pdl_launch_dependents();
-    const bool computes = wk < WK;              // (a copy warp takes part in the barriers and the sums)
-    if (computes)
 #pragma unroll
     for (int a = 0; a < WPL; ++a)
 #pragma unroll
