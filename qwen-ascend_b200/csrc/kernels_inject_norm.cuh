@@ -224,7 +224,7 @@ FNX_DEV float warp_sums32(float (&v)[32]) {
 // one the mean that the norm behind the block needs.
 // Bound: HBM, (4 HC + 2) * H * 2 bytes a token.
 template <int HC>
-__global__ void __launch_bounds__(512) inject_norm_bwd_kernel(const InjectNormBwdParams p) {
+__global__ void __launch_bounds__(512, HC == 1 ? 2 : 1) inject_norm_bwd_kernel(const InjectNormBwdParams p) {
     extern __shared__ __align__(128) uint8_t stages[];
     __shared__ float red[16][32], red1[16];
     __shared__ uint64_t full[2];
