@@ -1452,7 +1452,7 @@ int w4_dense_launch_t(const W4DenseParams& p, int CL, cudaStream_t st) {
     return launch_rc();
 }
 
-template <int NT>
+template <int NT, int SEG>
 int w4_dense_tma_launch_t(const W4DenseParams& d, int CL, cudaStream_t st) {
     EncodeTiledFn fn = encode_fn();
     if (!fn) return FNX_EDRIVER;
@@ -1479,7 +1479,7 @@ int w4_dense_tma_launch_t(const W4DenseParams& d, int CL, cudaStream_t st) {
     static bool configured[FNX_MAX_DEVICES] = {};
     const int dev = current_device();
     if (!configured[dev]) {
-        if (cudaFuncSetAttribute(w4_dense_tma_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        if (cudaFuncSetAttribute(w4_dense_tma_kernel<NT, SEG>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  113 * 1024) != cudaSuccess)   // every ring and sum (w4_tma_stages)
             return FNX_ELAUNCH;
         configured[dev] = true;
@@ -1498,8 +1498,15 @@ int w4_dense_tma_launch_t(const W4DenseParams& d, int CL, cudaStream_t st) {
     cfg.stream = st;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    if (cudaLaunchKernelEx(&cfg, w4_dense_tma_kernel<NT>, p) != cudaSuccess) return FNX_ELAUNCH;
+    if (cudaLaunchKernelEx(&cfg, w4_dense_tma_kernel<NT, SEG>, p) != cudaSuccess) return FNX_ELAUNCH;
     return launch_rc();
+}
+template <int NT>
+int w4_dense_tma_launch(const W4DenseParams& d, int CL, cudaStream_t st) {
+    if (d.gs % 128 == 0) return w4_dense_tma_launch_t<NT, 8>(d, CL, st);
+    if (d.gs == 64) return w4_dense_tma_launch_t<NT, 4>(d, CL, st);
+    if (d.gs == 32) return w4_dense_tma_launch_t<NT, 2>(d, CL, st);
+    return w4_dense_tma_launch_t<NT, 0>(d, CL, st);
 }
 }  // namespace
 
@@ -1529,7 +1536,7 @@ FNX_API int fnx_w4a16_gemv(const void* x, long long ld_x, const void* w4, const 
             const long long cost = per_sm * ((stages + c - 1) / c) + 3 * ((per_sm + 1) / 2) + (per_sm == 1 ? (stages + c - 1) / c / 2 : 0);
             if (cost < best) best = cost, C = c;
         }
-        return NT == 2 ? w4_dense_tma_launch_t<2>(p, C, st) : w4_dense_tma_launch_t<1>(p, C, st);
+        return NT == 2 ? w4_dense_tma_launch<2>(p, C, st) : w4_dense_tma_launch<1>(p, C, st);
     }
     if (NT == 2) return w4_dense_launch_t<1, 2>(p, CL, st);
     if (N % 16 == 0) return w4_dense_launch_t<2, 1>(p, CL, st);

@@ -272,7 +272,10 @@ __host__ __device__ inline int w4_tma_stage_bytes(int nt, int srows) {
     return W4T_W_BYTES + W4T_ROWS / 64 * nt * 1024 + (srows * 512 + 1023) / 1024 * 1024;      // x's boxes: 1 KB per 8 tokens and 64 k
 }
 
-template <int NT>
+// SEG: steps between two scalings where groups end at multiples of it in every warp's half of a stage
+// (gs 32, 64, or a multiple of 128: 2, 4, 8), so that the eight steps are one straight piece of code;
+// 0: wherever the group ends.
+template <int NT, int SEG>
 __global__ void __launch_bounds__(W4D_THREADS, 2) w4_dense_tma_kernel(const __grid_constant__ W4TmaParams q) {
     constexpr int WN = 4, WK = 2, STEPS = W4T_ROWS / 16 / WK;
     const W4DenseParams& p = q.d;
@@ -345,8 +348,9 @@ __global__ void __launch_bounds__(W4D_THREADS, 2) w4_dense_tma_kernel(const __gr
         if (!__all_sync(0xffffffffu, mbar_wait(&full[s], ph))) break;
         const uint8_t* S = base + s * stage_bytes;
         const int first = (s0 + j) * (W4T_ROWS / 16), mine = first + wk * STEPS;
-        int grp = group_of(mine);
-        int left = (grp + 1) * gsteps - mine;            // steps to the end of the group
+        int left = 0;                                    // steps to the end of the group
+        const int grp = group_of(mine);
+        if (SEG == 0) left = (grp + 1) * gsteps - mine;
         const uint8_t* sc = S + c0 + (grp - group_of(first)) * 512;
 #pragma unroll
         for (int u = 0; u < STEPS; ++u) {
@@ -366,7 +370,7 @@ __global__ void __launch_bounds__(W4D_THREADS, 2) w4_dense_tma_kernel(const __gr
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int n = 0; n < NT; ++n) mma_16816_bf16(acc[i][n], f[i][0], f[i][1], f[i][2], f[i][3], b[n][0], b[n][1]);
-            if (--left == 0 || u == STEPS - 1) {
+            if (SEG ? u % (SEG ? SEG : 1) == SEG - 1 : (--left == 0 || u == STEPS - 1)) {
                 const uint4 u4 = *reinterpret_cast<const uint4*>(sc);
                 const float v[8] = {bf_lo(u4.x), bf_hi(u4.x), bf_lo(u4.y), bf_hi(u4.y),
                                     bf_lo(u4.z), bf_hi(u4.z), bf_lo(u4.w), bf_hi(u4.w)};
