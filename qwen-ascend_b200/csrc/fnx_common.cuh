@@ -52,6 +52,10 @@ FNX_DEV uint64_t fnx_globaltimer() {
 
 FNX_DEV uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 
+// The next 1024-byte boundary in shared memory, by pointer arithmetic: through an integer the compiler
+// loses the address space and every access becomes a generic one with 64-bit addresses.
+FNX_DEV uint8_t* align1024(uint8_t* smem) { return smem + ((0u - smem_u32(smem)) & 1023u); }
+
 // ------------------------------------------------------------------ bf16 helpers
 FNX_DEV float bf2f(bf16 v) { return __bfloat162float(v); }
 FNX_DEV bf16 f2bf(float v) { return __float2bfloat16_rn(v); }

@@ -228,7 +228,7 @@ template <int EPI>
 __global__ void __launch_bounds__(FF_THREADS, 1) ffn_gemm_kernel(const __grid_constant__ FfnParams p) {
     constexpr int STAGES = ff_stages(EPI), BUFS = ff_epi_bufs(EPI);
     extern __shared__ __align__(1024) uint8_t smem_raw[];
-    uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* base = align1024(smem_raw);
     uint8_t* epi_buf = base + STAGES * FF_STAGE;
     FfnSmem& S = *reinterpret_cast<FfnSmem*>(epi_buf + FF_EPI_WARPS * BUFS * FF_EPI_BUF);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;

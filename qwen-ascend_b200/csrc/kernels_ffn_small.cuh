@@ -66,7 +66,7 @@ template <int EPI, int BN>
 __global__ void __launch_bounds__(FS_THREADS) ffn_small_kernel(const __grid_constant__ FfnSmallParams p) {
     constexpr int COLS = EPI == FF_GATED ? BN / 2 : BN;      // columns of the output per tile
     extern __shared__ __align__(1024) uint8_t smem_raw[];
-    uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* base = align1024(smem_raw);
     FfnSmallSmem& S = *reinterpret_cast<FfnSmallSmem*>(base + ffn_small_body(BN, p.a_rows, p.stages));
     float* sums = reinterpret_cast<float*>(base);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;

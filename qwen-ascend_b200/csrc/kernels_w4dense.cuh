@@ -280,7 +280,7 @@ __global__ void __launch_bounds__(W4D_THREADS, 2) w4_dense_tma_kernel(const __gr
     constexpr int WN = 4, WK = 2, STEPS = W4T_ROWS / 16 / WK;
     const W4DenseParams& p = q.d;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
-    uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* base = align1024(smem_raw);
     __shared__ uint64_t full[W4T_MAX_STAGES], empty[W4T_MAX_STAGES];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
