@@ -1453,13 +1453,12 @@ int w4_dense_launch_t(const W4DenseParams& p, int CL, cudaStream_t st) {
 }
 
 template <int NT, int SEG>
-int w4_dense_tma_launch_t(const W4DenseParams& d, int CL, cudaStream_t st) {
+int w4_dense_tma_launch_t(const W4DenseParams& d, cudaStream_t st) {
     EncodeTiledFn fn = encode_fn();
     if (!fn) return FNX_EDRIVER;
     W4TmaParams p;
     p.d = d;
     p.gshift = -1;
-    p.stages = 0;
     for (int b = 0; b < 20; ++b)
         if (d.gs == 16 << b) p.gshift = b;
     p.srows = d.gs % W4T_ROWS == 0 ? 1 : W4T_ROWS % d.gs == 0 ? W4T_ROWS / d.gs : (W4T_ROWS - 1) / d.gs + 2;
@@ -1477,6 +1476,7 @@ int w4_dense_tma_launch_t(const W4DenseParams& d, int CL, cudaStream_t st) {
              CU_TENSOR_MAP_SWIZZLE_NONE))
         return FNX_EALIGN;
     static bool configured[FNX_MAX_DEVICES] = {};
+    static int resident[FNX_MAX_DEVICES][9] = {};            // clusters of each size the device holds at once
     const int dev = current_device();
     if (!configured[dev]) {
         if (cudaFuncSetAttribute(w4_dense_tma_kernel<NT, SEG>, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -1487,26 +1487,52 @@ int w4_dense_tma_launch_t(const W4DenseParams& d, int CL, cudaStream_t st) {
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 1;
-    attr[0].val.clusterDim.y = (unsigned)CL;
     attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((d.N + W4D_FEATS - 1) / W4D_FEATS), (unsigned)CL, (unsigned)((d.M + 8 * NT - 1) / (8 * NT)));
     cfg.blockDim = dim3(W4D_THREADS, 1, 1);
     cfg.dynamicSmemBytes = w4_dense_tma_smem<NT>(d.M, p.srows);
     cfg.stream = st;
     cfg.attrs = attr;
+    const unsigned nt = (unsigned)((d.N + W4D_FEATS - 1) / W4D_FEATS), mt = (unsigned)((d.M + 8 * NT - 1) / (8 * NT));
+    // Parts of K, in units of one stage on an SM with two CTAs (three for a CTA's start and the cluster's
+    // sum; alone on an SM a CTA takes 1.5 a stage).  Whole rounds of the clusters that fit at once (which
+    // the GPCs' sizes limit: clusters of 6 leave slots empty), then the rest.
+    const int stages = (d.K + W4T_ROWS - 1) / W4T_ROWS;
+    const long long tiles = (long long)nt * mt;
+    int CL = 1;
+    double best = 1e30;
+    for (int c = 1; c <= 8 && c <= stages; ++c) {
+        int& fit = resident[dev][c];
+        if (!fit) {
+            attr[0].val.clusterDim.y = (unsigned)c;
+            cfg.gridDim = dim3(1, (unsigned)c, 1);
+            cfg.numAttrs = 1;
+            if (cudaOccupancyMaxActiveClusters(&fit, w4_dense_tma_kernel<NT, SEG>, &cfg) != cudaSuccess || fit < 1) {
+                cudaGetLastError();
+                fit = 1;
+            }
+        }
+        const double part = (stages + c - 1) / c;
+        const long long rest = tiles % fit;
+        const double cost = (double)(tiles / fit) * (2 * part + 3) +
+                            (rest ? (rest * c > num_sms() ? 2 : 1.5) * part + 3 : 0);
+        if (cost < best) best = cost, CL = c;
+    }
+    attr[0].val.clusterDim.y = (unsigned)CL;
+    cfg.gridDim = dim3(nt, (unsigned)CL, mt);
     cfg.numAttrs = 2;
     if (cudaLaunchKernelEx(&cfg, w4_dense_tma_kernel<NT, SEG>, p) != cudaSuccess) return FNX_ELAUNCH;
     return launch_rc();
 }
+
 template <int NT>
-int w4_dense_tma_launch(const W4DenseParams& d, int CL, cudaStream_t st) {
-    if (d.gs % 128 == 0) return w4_dense_tma_launch_t<NT, 8>(d, CL, st);
-    if (d.gs == 64) return w4_dense_tma_launch_t<NT, 4>(d, CL, st);
-    if (d.gs == 32) return w4_dense_tma_launch_t<NT, 2>(d, CL, st);
-    return w4_dense_tma_launch_t<NT, 0>(d, CL, st);
+int w4_dense_tma_launch(const W4DenseParams& d, cudaStream_t st) {
+    if (d.gs % 128 == 0) return w4_dense_tma_launch_t<NT, 8>(d, st);
+    if (d.gs == 64) return w4_dense_tma_launch_t<NT, 4>(d, st);
+    if (d.gs == 32) return w4_dense_tma_launch_t<NT, 2>(d, st);
+    return w4_dense_tma_launch_t<NT, 0>(d, st);
 }
 }  // namespace
 
@@ -1519,25 +1545,15 @@ FNX_API int fnx_w4a16_gemv(const void* x, long long ld_x, const void* w4, const 
     if (!aligned16(x) || !aligned16(w4) || !aligned16(scales) || !aligned16(y) || ld_x % 4) return FNX_EALIGN;
     const W4DenseParams p{(const bf16*)x, (const uint32_t*)w4, (const bf16*)scales, (bf16*)y, ld_x, M, K, N, gs};
     const int NT = M <= 8 ? 1 : 2;
+    cudaStream_t st = (cudaStream_t)stream;
+    // from 8 MB of weights on the ring of TMA copies (2048 x 16384, 8 tokens: 8.1 us against 15.6); below,
+    // the two are within a microsecond and the direct loads need no tensor maps (1.4 us of host time)
+    if (N % 32 == 0 && ld_x % 8 == 0 && (long long)K * N >= 16 << 20)
+        return NT == 2 ? w4_dense_tma_launch<2>(p, st) : w4_dense_tma_launch<1>(p, st);
+    // parts of K until the CTAs fill the SMs twice, at least 16 steps of 16 rows each
     const long long tiles = (long long)((N + W4D_FEATS - 1) / W4D_FEATS) * ((M + 8 * NT - 1) / (8 * NT));
     int CL = 1;
     while (CL < 8 && tiles * CL < 2 * num_sms() && K / (16 * CL) >= 16) CL *= 2;
-    cudaStream_t st = (cudaStream_t)stream;
-    // from 8 MB of weights on the ring of TMA copies (2048 x 16384, 8 tokens: 10.0 us against 15.6); below,
-    // the two are within 0.3 us of each other and the direct loads need no tensor maps (1.4 us of host time)
-    if (N % 32 == 0 && ld_x % 8 == 0 && (long long)K * N >= 16 << 20) {
-        // parts of K: the SM with the most CTAs works through its stages one after another, and every
-        // part costs a start and the cluster's sum (about three stages)
-        const int stages = (K + W4T_ROWS - 1) / W4T_ROWS;
-        int C = 1;
-        long long best = 1LL << 60;
-        for (int c = 1; c <= 8 && c <= stages; ++c) {
-            const long long per_sm = (tiles * c + num_sms() - 1) / num_sms();
-            const long long cost = per_sm * ((stages + c - 1) / c) + 3 * ((per_sm + 1) / 2) + (per_sm == 1 ? (stages + c - 1) / c / 2 : 0);
-            if (cost < best) best = cost, C = c;
-        }
-        return NT == 2 ? w4_dense_tma_launch<2>(p, C, st) : w4_dense_tma_launch<1>(p, C, st);
-    }
     if (NT == 2) return w4_dense_launch_t<1, 2>(p, CL, st);
     if (N % 16 == 0) return w4_dense_launch_t<2, 1>(p, CL, st);
     return w4_dense_launch_t<1, 1>(p, CL, st);
