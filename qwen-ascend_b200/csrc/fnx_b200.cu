@@ -1343,17 +1343,20 @@ int ffn_products(const FfnGemm* g, int count, float* gu, bool chained, bool foll
         if (g[i].amn) box_rows = 128;
         else if (g[i].M > box_rows) box_rows = g[i].M;
     }
-    // Few rows: the weights' bytes are the work, 128-row tiles of them.  More rows: 64 columns, while
-    // the tiles fit the SMs twice; beyond that CTA pairs, unless their 256 rows would be half empty.
-    const bool few = rows <= 32, fits = t64 <= 256;
+    // Few rows: the weights' bytes are the work, 128-row tiles of them (64 where even eight parts of K
+    // leave SMs free).  More rows: 64 columns, while the tiles fit the SMs twice; beyond that CTA pairs,
+    // unless their 256 rows would be half empty.
+    const bool few = rows <= 64, fits = t64 <= 256;
     if (!few && !fits && rows > 128) return ffn_pair_launch<EPI>(g, count, gu, followed, st);
-    const int BN = few || !fits ? 128 : 64;
+    const int BN = few ? (t64 * FS_MAX_CL <= num_sms() ? 64 : 128) : fits ? 64 : 128;
     const long long tiles = BN == 64 ? t64 : t128;
     if (tiles > 0x7ffffffLL) return FNX_ESHAPE;
-    // parts of K while the CTAs fit the SMs twice, at least four k-blocks each (a part costs the
-    // cluster's sum: 2 k-blocks each took 10.2 us where 4 took 7.5, 128 x 1024 x 2048)
+    // parts of K while the CTAs fit the SMs twice (clusters of more than two leave some of a GPC's slots
+    // empty: 264 of 296), at least four k-blocks each (a part costs the cluster's sum: two k-blocks each
+    // took 10.2 us where four took 7.5, 128 x 1024 x 2048)
     int CL = 1;
-    while (CL < FS_MAX_CL && 2 * CL * tiles <= 2LL * num_sms() && KB / (2 * CL) >= 4) CL *= 2;
+    for (int c = 2; c <= FS_MAX_CL; ++c)
+        if (c * tiles <= (c == 2 ? 2LL * num_sms() : 264LL * num_sms() / 148) && KB / c >= 4) CL = c;
     int a_rows = 128;
     while (a_rows > 16 && a_rows / 2 >= box_rows) a_rows /= 2;
     int stages = 92 * 1024 / ((a_rows + BN) * 128);          // a ring that leaves room for a second CTA on the SM
@@ -1418,6 +1421,18 @@ FNX_API int fnx_gated_ffn_backward(const void* dy, long long ld_dy, const void* 
     if (dx) g[n++] = FfnGemm{dgu, w_gu, dx, nullptr, 2LL * I, H, H, M, H, 2 * I, 0, 1};
     if (dw_gu) g[n++] = FfnGemm{dgu, x, dw_gu, nullptr, 2LL * I, ld_x, H, 2 * I, H, M, 1, 1};
     if (dw_down) g[n++] = FfnGemm{dy, h, dw_down, nullptr, ld_dy, I, I, O, I, M, 1, 1};
+    // dx on its own where its few tiles are long sums (K = 2I) beside short ones (K = M): in one launch with
+    // the weight gradients its parts of K would be theirs, and its last tile the launch's end, by more than
+    // a launch costs (about 24 k-blocks; 83 rows of 552 x 5400: 84 -> 49 us, 509 of 2048 x 512: 36 -> 42)
+    if (dx && n > 1) {
+        long long blocks = 0;                         // k-blocks of all 256 x 256 tiles
+        for (int i = 0; i < n; ++i)
+            blocks += (long long)((g[i].M + 255) / 256) * ((g[i].N + 255) / 256) * ((g[i].K + FF_BK - 1) / FF_BK);
+        if (((2LL * I + FF_BK - 1) / FF_BK - 24) * (num_sms() / 2) > blocks) {
+            rc = ffn_products<FF_PLAIN>(g, 1, nullptr, true, false, st);
+            return rc ? rc : ffn_products<FF_PLAIN>(g + 1, n - 1, nullptr, true, false, st);
+        }
+    }
     if (n) rc = ffn_products<FF_PLAIN>(g, n, nullptr, true, false, st);
     return rc;
 }
