@@ -1467,7 +1467,7 @@ int w4_dense_launch_t(const W4DenseParams& p, int CL, cudaStream_t st) {
     return launch_rc();
 }
 
-template <int NT, int SEG>
+template <int NT, int SEG, int QUAD>
 int w4_dense_tma_launch_t(const W4DenseParams& d, cudaStream_t st) {
     EncodeTiledFn fn = encode_fn();
     if (!fn) return FNX_EDRIVER;
@@ -1485,7 +1485,9 @@ int w4_dense_tma_launch_t(const W4DenseParams& d, cudaStream_t st) {
         return fn(m, dt, 2, const_cast<void*>(ptr), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
     };
-    if (!map(&p.tw, CU_TENSOR_MAP_DATA_TYPE_INT32, d.w, d.N / 8, d.K, d.N / 2, 32, W4T_ROWS, CU_TENSOR_MAP_SWIZZLE_128B) ||
+    constexpr int RQ = QUAD ? 4 : 1;                         // rows seen as one
+    if (!map(&p.tw, CU_TENSOR_MAP_DATA_TYPE_INT32, d.w, (unsigned long long)RQ * (d.N / 8), d.K / RQ, RQ * (d.N / 2ull), 32,
+             W4T_ROWS / RQ, CU_TENSOR_MAP_SWIZZLE_128B) ||
         !map(&p.tx, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, d.x, d.K, d.M, d.ld_x * 2, 64, 8 * NT, CU_TENSOR_MAP_SWIZZLE_128B) ||
         !map(&p.ts, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, d.s, d.N, (d.K + d.gs - 1) / d.gs, d.N * 2ull, W4D_FEATS, p.srows,
              CU_TENSOR_MAP_SWIZZLE_NONE))
@@ -1494,7 +1496,7 @@ int w4_dense_tma_launch_t(const W4DenseParams& d, cudaStream_t st) {
     static int resident[FNX_MAX_DEVICES][9] = {};            // clusters of each size the device holds at once
     const int dev = current_device();
     if (!configured[dev]) {
-        if (cudaFuncSetAttribute(w4_dense_tma_kernel<NT, SEG>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        if (cudaFuncSetAttribute(w4_dense_tma_kernel<NT, SEG, QUAD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  113 * 1024) != cudaSuccess)   // every ring and sum (w4_tma_stages)
             return FNX_ELAUNCH;
         configured[dev] = true;
@@ -1510,7 +1512,8 @@ int w4_dense_tma_launch_t(const W4DenseParams& d, cudaStream_t st) {
     cfg.dynamicSmemBytes = w4_dense_tma_smem<NT>(d.M, p.srows);
     cfg.stream = st;
     cfg.attrs = attr;
-    const unsigned nt = (unsigned)((d.N + W4D_FEATS - 1) / W4D_FEATS), mt = (unsigned)((d.M + 8 * NT - 1) / (8 * NT));
+    constexpr int FEATS = QUAD ? 224 : 256;
+    const unsigned nt = (unsigned)((d.N + FEATS - 1) / FEATS), mt = (unsigned)((d.M + 8 * NT - 1) / (8 * NT));
     // Parts of K, in units of one stage on an SM with two CTAs (three for a CTA's start and the cluster's
     // sum; alone on an SM a CTA takes 1.5 a stage).  Whole rounds of the clusters that fit at once (which
     // the GPCs' sizes limit: clusters of 6 leave slots empty), then the rest.
@@ -1524,7 +1527,7 @@ int w4_dense_tma_launch_t(const W4DenseParams& d, cudaStream_t st) {
             attr[0].val.clusterDim.y = (unsigned)c;
             cfg.gridDim = dim3(1, (unsigned)c, 1);
             cfg.numAttrs = 1;
-            if (cudaOccupancyMaxActiveClusters(&fit, w4_dense_tma_kernel<NT, SEG>, &cfg) != cudaSuccess || fit < 1) {
+            if (cudaOccupancyMaxActiveClusters(&fit, w4_dense_tma_kernel<NT, SEG, QUAD>, &cfg) != cudaSuccess || fit < 1) {
                 cudaGetLastError();
                 fit = 1;
             }
@@ -1538,16 +1541,20 @@ int w4_dense_tma_launch_t(const W4DenseParams& d, cudaStream_t st) {
     attr[0].val.clusterDim.y = (unsigned)CL;
     cfg.gridDim = dim3(nt, (unsigned)CL, mt);
     cfg.numAttrs = 2;
-    if (cudaLaunchKernelEx(&cfg, w4_dense_tma_kernel<NT, SEG>, p) != cudaSuccess) return FNX_ELAUNCH;
+    if (cudaLaunchKernelEx(&cfg, w4_dense_tma_kernel<NT, SEG, QUAD>, p) != cudaSuccess) return FNX_ELAUNCH;
     return launch_rc();
 }
 
+template <int NT, int QUAD>
+int w4_dense_tma_launch(const W4DenseParams& d, cudaStream_t st) {
+    if (d.gs % 128 == 0) return w4_dense_tma_launch_t<NT, 8, QUAD>(d, st);
+    if (d.gs == 64) return w4_dense_tma_launch_t<NT, 4, QUAD>(d, st);
+    if (d.gs == 32) return w4_dense_tma_launch_t<NT, 2, QUAD>(d, st);
+    return w4_dense_tma_launch_t<NT, 0, QUAD>(d, st);
+}
 template <int NT>
 int w4_dense_tma_launch(const W4DenseParams& d, cudaStream_t st) {
-    if (d.gs % 128 == 0) return w4_dense_tma_launch_t<NT, 8>(d, st);
-    if (d.gs == 64) return w4_dense_tma_launch_t<NT, 4>(d, st);
-    if (d.gs == 32) return w4_dense_tma_launch_t<NT, 2>(d, st);
-    return w4_dense_tma_launch_t<NT, 0>(d, st);
+    return d.N % 32 == 0 ? w4_dense_tma_launch<NT, 0>(d, st) : w4_dense_tma_launch<NT, 1>(d, st);
 }
 }  // namespace
 
@@ -1561,9 +1568,11 @@ FNX_API int fnx_w4a16_gemv(const void* x, long long ld_x, const void* w4, const 
     const W4DenseParams p{(const bf16*)x, (const uint32_t*)w4, (const bf16*)scales, (bf16*)y, ld_x, M, K, N, gs};
     const int NT = M <= 8 ? 1 : 2;
     cudaStream_t st = (cudaStream_t)stream;
-    // from 8 MB of weights on the ring of TMA copies (2048 x 16384, 8 tokens: 8.1 us against 15.6); below,
-    // the two are within a microsecond and the direct loads need no tensor maps (1.4 us of host time)
-    if (N % 32 == 0 && ld_x % 8 == 0 && (long long)K * N >= 16 << 20)
+    // From 8 MB of weights on the ring of TMA copies (2048 x 16384, 8 tokens: 8.1 us against 15.6; 6352 x
+    // 13768, whose rows are off 16 bytes: 17.6 against 27.5).  Below, the direct loads: the ring is about
+    // 1 us faster on the GPU (2048 x 5120: 4.9 against 5.8) but its tensor maps cost the host that much
+    // and more (a call by itself: 11.9 us against 10.4), which such a short call waits for.
+    if (ld_x % 8 == 0 && (long long)K * N >= 16 << 20)
         return NT == 2 ? w4_dense_tma_launch<2>(p, st) : w4_dense_tma_launch<1>(p, st);
     // parts of K until the CTAs fill the SMs twice, at least 16 steps of 16 rows each
     const long long tiles = (long long)((N + W4D_FEATS - 1) / W4D_FEATS) * ((M + 8 * NT - 1) / (8 * NT));

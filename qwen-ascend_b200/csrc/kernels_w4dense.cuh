@@ -7,15 +7,19 @@
 // bf16(q * s), what the grouped GEMM multiplies with, would cost a rounding per weight and an
 // instruction more.
 //
-// Bound: the weight stream, K * N / 2 bytes read once.  The products run on mma.sync m16n8k16, which
-// is far from its rate at this traffic: weights are the 16-row operand straight from registers, the
-// tokens the 8-column one.  A lane loads one or two words of four consecutive rows k; a byte permute
-// brings the same byte of two rows' words into the two halves of a register, whose nibbles are then the
-// (k, k+1) pairs that the fragments want (nib_lo, nib_hi).  The order of k inside a fragment is free as long as the tokens use the same one: lane t of a fragment
-// group takes rows 4t .. 4t+3 of a 16-row step, so its tokens are one 8-byte load.
-// Split: a warp takes 64 * WPL features; eight warps of a CTA split 4 / 2 over K and the rest over
-// features; the CTAs of a cluster split K again and add their parts through distributed shared
-// memory in a fixed order (deterministic).
+// Bound: the weight stream, K * N / 2 bytes read once, at long streams the issue of its conversion (8192 x
+// 28672, groups of 128, one token: 33.8 us, 3.6 TB/s of weights and scales; 4096 x 28672, groups of 32,
+// 16 tokens: 28.0 us), at short ones a launch and the cluster's sum (2048 x 5120, one token: 5.8 us).
+// The products run on mma.sync m16n8k16, which is far from its rate at this traffic (19 % busy): weights
+// are the 16-row operand straight from registers, the tokens the 8-column one.  A byte permute brings
+// the same byte of two rows' words into the two halves of a register, whose nibbles are then the (k, k+1)
+// pairs that the fragments want (nib_lo, nib_hi).
+// Split: the warps of a CTA split its 256 features (224: see QUAD) and K; the CTAs of a cluster split K
+// again and add their parts through distributed shared memory in a fixed order (deterministic).
+//
+// w4_dense_kernel, short streams: a lane loads one or two words of four consecutive rows k, rows 4t ..
+// 4t+3 of a 16-row step (the order of k inside a fragment is free as long as the tokens use the same
+// one), so its tokens are one 8-byte load.
 #pragma once
 #include "fnx_common.cuh"
 
@@ -67,10 +71,11 @@ struct W4DenseParams {
 };
 
 // Adds the parts of the CTA's warps, then of the cluster's CTAs, in order, and writes y.  red: [WK][mt][W4D_FEATS].
-template <int WPL, int NT>
+template <int WPL, int NT, int FEATS>
 FNX_DEV void w4_dense_finish(const W4DenseParams& p, const float (&tot)[WPL][4][NT][4], float* red, int wn, int wk, int g,
                              int t, uint32_t rank, int CL, int m0, int mt) {
-    constexpr int WF = 64 * WPL, WK = 8 / (W4D_FEATS / WF);
+    constexpr int WF = 64 * WPL, WN = W4D_FEATS / WF, WK = 8 / WN;
+    constexpr int WW = FEATS / 8 / WN;          // words of a warp (lanes beyond them hold nothing)
     pdl_launch_dependents();
 #pragma unroll
     for (int a = 0; a < WPL; ++a)
@@ -79,8 +84,8 @@ FNX_DEV void w4_dense_finish(const W4DenseParams& p, const float (&tot)[WPL][4][
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 const int tok = n * 8 + 2 * t + c;
-                if (tok < mt) {
-                    float* o = red + ((size_t)wk * mt + tok) * W4D_FEATS + wn * WF + (g * WPL + a) * 8;
+                if (tok < mt && g * WPL + a < WW) {
+                    float* o = red + ((size_t)wk * mt + tok) * FEATS + (wn * WW + g * WPL + a) * 8;
                     *reinterpret_cast<float4*>(o) = make_float4(tot[a][0][n][c], tot[a][1][n][c], tot[a][2][n][c],
                                                                 tot[a][3][n][c]);
                     *reinterpret_cast<float4*>(o + 4) = make_float4(tot[a][0][n][2 + c], tot[a][1][n][2 + c],
@@ -88,7 +93,7 @@ FNX_DEV void w4_dense_finish(const W4DenseParams& p, const float (&tot)[WPL][4][
                 }
             }
     __syncthreads();
-    const int cells = mt * W4D_FEATS;
+    const int cells = mt * FEATS;
     for (int i = threadIdx.x; i < cells; i += blockDim.x) {
         float v = red[i];
 #pragma unroll
@@ -98,7 +103,7 @@ FNX_DEV void w4_dense_finish(const W4DenseParams& p, const float (&tot)[WPL][4][
     if (CL > 1) cluster_sync_all(); else __syncthreads();
     const int per = (cells / 2 + CL - 1) / CL;                  // pairs of features of this CTA
     for (int i = (int)rank * per + threadIdx.x; i < min(cells / 2, (int)(rank + 1) * per); i += blockDim.x) {
-        const int tok = 2 * i / W4D_FEATS, f = blockIdx.x * W4D_FEATS + 2 * i % W4D_FEATS;
+        const int tok = 2 * i / FEATS, f = blockIdx.x * FEATS + 2 * i % FEATS;
         if (f >= p.N) continue;
         float2 v = *reinterpret_cast<const float2*>(red + 2 * i);
         if (CL > 1) {
@@ -241,7 +246,7 @@ __global__ void __launch_bounds__(W4D_THREADS, 2) w4_dense_kernel(const W4DenseP
         if (left != gsteps) scale(grp);
     }
 
-    w4_dense_finish<WPL, NT>(p, tot, red, wn, wk, g, t, rank, CL, m0, mt);
+    w4_dense_finish<WPL, NT, W4D_FEATS>(p, tot, red, wn, wk, g, t, rank, CL, m0, mt);
 }
 
 template <int WPL, int NT>
@@ -250,7 +255,7 @@ inline size_t w4_dense_smem(int M) {
     return (size_t)WK * (M < 8 * NT ? M : 8 * NT) * W4D_FEATS * sizeof(float);
 }
 
-// The same sums for long weight streams (N % 32 == 0): a ring of two or three stages of 256 rows x 256
+// The same sums for long weight streams: a ring of two or three stages of 256 rows x 256
 // features kept in flight by TMA, with the tokens' 256 columns and the stage's scale rows, so neither
 // the stream's depth nor a scale's latency is the warps' concern.  With the 128-byte swizzle the
 // fragment loads are free of bank conflicts for the natural order of k (lane t: rows 2t, 2t+1, 2t+8,
@@ -275,9 +280,14 @@ __host__ __device__ inline int w4_tma_stage_bytes(int nt, int srows) {
 // SEG: steps between two scalings where groups end at multiples of it in every warp's half of a stage
 // (gs 32, 64, or a multiple of 128: 2, 4, 8), so that the eight steps are one straight piece of code;
 // 0: wherever the group ends.
-template <int NT, int SEG>
+// QUAD: where N % 32 != 0 a row does not start on the 16 bytes that a copy needs.  Four rows together do,
+// so the copies see K / 4 rows of four, one box for each row j of the four, from the 16 bytes below its
+// first word (d_j = j * N / 8 mod 4 words further down); 28 words of a box's 32 are then the tile's,
+// whichever d_j.  What a box holds beyond a row's end belongs to features that are not stored.
+template <int NT, int SEG, int QUAD>
 __global__ void __launch_bounds__(W4D_THREADS, 2) w4_dense_tma_kernel(const __grid_constant__ W4TmaParams q) {
     constexpr int WN = 4, WK = 2, STEPS = W4T_ROWS / 16 / WK;
+    constexpr int TW = QUAD ? 28 : 32, WW = TW / WN;     // words of a tile and of a warp
     const W4DenseParams& p = q.d;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* base = align1024(smem_raw);
@@ -308,11 +318,17 @@ __global__ void __launch_bounds__(W4D_THREADS, 2) w4_dense_tma_kernel(const __gr
         const int row = (s0 + j) * W4T_ROWS;
         const uint32_t w = smem_u32(base + s * stage_bytes);
         mbar_arrive_expect_tx(&full[s], W4T_W_BYTES + W4T_ROWS / 64 * NT * 1024 + q.srows * 512);
-        tma_load_2d(w, &q.tw, &full[s], blockIdx.x * (W4D_FEATS / 8), row);
+        if (QUAD) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                tma_load_2d(w + i * (W4T_W_BYTES / 4), &q.tw, &full[s], (i * (p.N / 8) + (int)blockIdx.x * TW) & ~3, row / 4);
+        } else {
+            tma_load_2d(w, &q.tw, &full[s], blockIdx.x * TW, row);
+        }
 #pragma unroll
         for (int i = 0; i < W4T_ROWS / 64; ++i)
             tma_load_2d(w + W4T_W_BYTES + i * NT * 1024, &q.tx, &full[s], row + 64 * i, m0);
-        tma_load_2d(w + W4T_W_BYTES + W4T_ROWS / 64 * NT * 1024, &q.ts, &full[s], blockIdx.x * W4D_FEATS,
+        tma_load_2d(w + W4T_W_BYTES + W4T_ROWS / 64 * NT * 1024, &q.ts, &full[s], blockIdx.x * (TW * 8),
                     group_of((s0 + j) * (W4T_ROWS / 16)));
     };
     if (warp == 0) {
@@ -331,9 +347,27 @@ __global__ void __launch_bounds__(W4D_THREADS, 2) w4_dense_tma_kernel(const __gr
     // offsets in a stage: the words of rows 2t and 2t+1 of this warp's first step (rows 8 further are
     // 1024 bytes on, steps 2048), the tokens' words of its first eight k (eight k further: another
     // 16-byte chunk, its index exchanged with the row's by the swizzle)
-    const int word = wn * 8 + g;
-    const uint32_t w0 = wk * STEPS * 2048 + (2 * t) * 128 + (((word >> 2) ^ ((2 * t) & 7)) << 4) + (word & 3) * 4;
-    const uint32_t w1 = wk * STEPS * 2048 + (2 * t + 1) * 128 + (((word >> 2) ^ ((2 * t + 1) & 7)) << 4) + (word & 3) * 4;
+    const int word = wn * WW + min(g, WW - 1);
+    uint32_t w0, w1;
+    if (QUAD) {                                          // row r of a step: box r % 4, its row 4 step + r / 4
+        auto at = [&](int r) {
+            const int d = word + (((r & 3) * (p.N / 8)) & 3);
+            return (r & 3) * (W4T_W_BYTES / 4) + (wk * STEPS * 4 + (r >> 2)) * 128 + (((d >> 2) ^ (r >> 2)) << 4) + (d & 3) * 4;
+        };
+        w0 = at(2 * t);
+        w1 = at(2 * t + 1);
+    } else {
+        auto at = [&](int r) {
+            return wk * STEPS * 2048 + r * 128 + (((word >> 2) ^ r) << 4) + (word & 3) * 4;
+        };
+        w0 = at(2 * t);
+        w1 = at(2 * t + 1);
+    }
+    // word i (row 2t, 2t+1, 2t+8, 2t+9) of step u
+    auto word_at = [&](int u, int i) {
+        const uint32_t o = i & 1 ? w1 : w0;
+        return QUAD ? (o ^ (((4 * u + (i & 2)) & 7) << 4)) + u * 512 + (i & 2) * 128 : o + u * 2048 + (i & 2) * 512;
+    };
     const uint32_t x0 = W4T_W_BYTES + wk * (STEPS / 4) * NT * 1024 + g * 128 + (g << 4) + t * 4;
     const uint32_t c0 = W4T_W_BYTES + W4T_ROWS / 64 * NT * 1024 + word * 16;
 
@@ -355,10 +389,8 @@ __global__ void __launch_bounds__(W4D_THREADS, 2) w4_dense_tma_kernel(const __gr
 #pragma unroll
         for (int u = 0; u < STEPS; ++u) {
             uint32_t wv[4], b[NT][2];
-            wv[0] = *reinterpret_cast<const uint32_t*>(S + w0 + u * 2048);
-            wv[1] = *reinterpret_cast<const uint32_t*>(S + w1 + u * 2048);
-            wv[2] = *reinterpret_cast<const uint32_t*>(S + w0 + u * 2048 + 1024);
-            wv[3] = *reinterpret_cast<const uint32_t*>(S + w1 + u * 2048 + 1024);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) wv[i] = *reinterpret_cast<const uint32_t*>(S + word_at(u, i));
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -392,7 +424,7 @@ __global__ void __launch_bounds__(W4D_THREADS, 2) w4_dense_tma_kernel(const __gr
         if (++s == NS) s = 0, ph ^= 1;
     }
     __syncthreads();                                     // every stage is read: the sums reuse the ring
-    w4_dense_finish<1, NT>(p, tot, reinterpret_cast<float*>(base), wn, wk, g, t, rank, CL, m0, mt);
+    w4_dense_finish<1, NT, TW * 8>(p, tot, reinterpret_cast<float*>(base), wn, wk, g, t, rank, CL, m0, mt);
 }
 
 // Stages of the ring: as many as leave room for two CTAs on an SM, at least two.
