@@ -49,8 +49,10 @@ def test_matches_the_definition(M, K, N, gs):
     check(lay, w, s, gs, torch.randn(M, K, generator=g).to(BF16).to(DEV))
 
 
-# from 2^24 weights on they come through the ring of copies: ragged K and N, groups that end inside a stage
+# from 2^24 weights on they come through the ring of copies: ragged K, every N mod 32, groups that end
+# inside a stage
 @pytest.mark.parametrize("M,K,N,gs", [(9, 5000, 4128, 48), (1, 4104, 4128, 16), (5, 8200, 2080, 4096), (17, 4096, 4104, 32),
+                                      (3, 4200, 4112, 64), (12, 4104, 4120, 128), (2, 8408, 2008, 256),
                                       (1, 8192, 28672, 128), (16, 4096, 14336, 32), (3, 2560, 151936, 64)])
 def test_wide(M, K, N, gs):
     lay, w, s = layer(K, N, gs)
