@@ -1182,7 +1182,7 @@ FNX_API int fnx_bf16_gemm_nt(const void* x, long long ld_x, const void* w, void*
 // ======================================================================== gated feed-forward block
 namespace {
 // A bf16 matrix as an operand or output of the block's products: `cols` contiguous elements per row,
-// rows `ld` elements apart.  Encoded per call (no cache: half a microsecond of host time).
+// rows `ld` elements apart.  Encoded per call (0.04 us of host time).
 int ffn_map(CUtensorMap* out, const void* ptr, long long cols, long long rows, long long ld, unsigned b0,
             unsigned b1) {
     EncodeTiledFn fn = encode_fn();
@@ -1569,9 +1569,9 @@ FNX_API int fnx_w4a16_gemv(const void* x, long long ld_x, const void* w4, const 
     const int NT = M <= 8 ? 1 : 2;
     cudaStream_t st = (cudaStream_t)stream;
     // From 8 MB of weights on the ring of TMA copies (2048 x 16384, 8 tokens: 8.1 us against 15.6; 6352 x
-    // 13768, whose rows are off 16 bytes: 17.6 against 27.5).  Below, the direct loads: the ring is about
-    // 1 us faster on the GPU (2048 x 5120: 4.9 against 5.8) but its tensor maps cost the host that much
-    // and more (a call by itself: 11.9 us against 10.4), which such a short call waits for.
+    // 13768, whose rows are off 16 bytes: 17.6 against 27.5).  Below, the direct loads: the ring takes
+    // about 1 us less on the GPU (2048 x 5120: 4.9 against 5.8) but a call from Python half a microsecond
+    // more (4096 x 2560: 8.8 against 8.2), and that is what such a short call waits for.
     if (ld_x % 8 == 0 && (long long)K * N >= 16 << 20)
         return NT == 2 ? w4_dense_tma_launch<2>(p, st) : w4_dense_tma_launch<1>(p, st);
     // parts of K until the CTAs fill the SMs twice, at least 16 steps of 16 rows each

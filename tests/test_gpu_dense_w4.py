@@ -139,6 +139,21 @@ def test_inputs_written_just_before_and_just_after_a_call(K, N):
         assert torch.equal(y, ya if i % 2 else yb)
 
 
+def test_offsets_past_32_bits():
+    """2^31 words and more: the last rows and columns are the ones that a 32-bit offset would miss."""
+    from fnx.engine import DenseW4
+    K, N, gs = 65536, 263168, 4096
+    w = torch.empty(K, N // 8, dtype=torch.int32, device=DEV).random_(-2 ** 31, 2 ** 31 - 1)
+    s = torch.full((K // gs, N), 0.01, dtype=BF16, device=DEV)
+    x = torch.randn(1, K, generator=torch.Generator().manual_seed(1)).to(BF16).to(DEV)
+    y = DenseW4(w, s, gs)(x)
+    for j in (0, 1, N // 16, N // 8 - 2, N // 8 - 1):
+        W = values64(w[:, j:j + 1].cpu(), s[:, 8 * j:8 * j + 8].cpu(), gs).to(DEV)
+        want, mag = x.double() @ W, x.double().abs() @ W.abs()
+        lim = 2 ** -8 * want.abs() + (K / 16 + K // gs + 64) * 2 ** -22 * mag
+        assert bool(((y[:, 8 * j:8 * j + 8].double() - want).abs() <= lim).all())
+
+
 def test_agrees_with_the_expert_gemm():
     """The same words as one expert of ExpW4, whose weights are rounded to bf16 first (2^-9 each on
     average): the two agree within the layer contract's relative L2 of 5e-3."""

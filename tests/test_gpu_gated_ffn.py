@@ -223,6 +223,29 @@ def test_inputs_and_weights_written_just_before_and_just_after_a_call(M, H, I):
         assert torch.equal(y, want[0][1])
 
 
+def test_offsets_past_32_bits():
+    """More than 2^31 elements of output, of kept pre-activations and of their gradients."""
+    f, _, _ = make(1, 64, 2056, 1032, 9)
+    M = 2 ** 20 + 77
+    x = torch.zeros(M, 64, dtype=BF16, device=DEV)
+    dy = torch.zeros(M, 1032, dtype=BF16, device=DEV)
+    g = torch.Generator().manual_seed(9)
+    for at in (0, M // 2, M - 200):
+        x[at:at + 200] = torch.randn(200, 64, generator=g).to(BF16).to(DEV)
+        dy[at:at + 200] = torch.randn(200, 1032, generator=g).to(BF16).to(DEV)
+    h = f.gated(x)
+    assert h.numel() > 2 ** 31
+    for at in (0, M // 2, M - 200):
+        close(h[at:at + 200], definition(f, x[at:at + 200])["h"], "h")
+    del h
+    y, saved = f.forward_train(x)
+    dx = f.backward(dy, saved, need=(True, False, False))[0]
+    for at in (0, M // 2, M - 200):
+        want = definition(f, x[at:at + 200], dy[at:at + 200])
+        close(y[at:at + 200], want["y"], "y")
+        close(dx[at:at + 200], want["dx"], "dx")
+
+
 def test_no_device_error_was_recorded():
     from fnx import _lib
     assert _lib.device_errors() == 0

@@ -188,6 +188,27 @@ def test_backward_is_deterministic_and_replays_from_a_graph():
         assert torch.equal(w, x)
 
 
+def test_offsets_past_32_bits():
+    from fnx.native_inject import inject_norm, inject_norm_backward
+    H, HC = 2048, 4
+    T = 2 ** 18 + 5
+    few = inputs(3, H, HC, 41)
+    where = torch.tensor([0, T // 2, T - 1], device=DEV)
+    big = []
+    for t in few[:3]:
+        b = torch.zeros(T, *t.shape[1:], dtype=BF16, device=DEV)
+        b[where] = t
+        big.append(b)
+    assert big[0].numel() > 2 ** 31
+    state, normed = inject_norm(big[0], big[1], big[2], few[3], w_post=few[4])
+    want = inject_norm(few[0], few[1], few[2], few[3], w_post=few[4])
+    assert torch.equal(state[where], want[0]) and torch.equal(normed[where], want[1])
+    got = inject_norm_backward(state, None, state, big[1], big[2], few[3], w_post=few[4])
+    want = inject_norm_backward(want[0], None, want[0], few[1], few[2], few[3], w_post=few[4])
+    for a, b in zip(got[:3], want[:3]):
+        assert torch.equal(a[where], b)
+
+
 def test_state_feeds_the_next_mix():
     """The fused step in the place of inject + the norm that opens gated_residual."""
     from fnx.engine import gated_residual
