@@ -1489,11 +1489,12 @@ int w4_dense_tma_launch_t(const W4DenseParams& d, cudaStream_t st) {
     if (!map(&p.tw, CU_TENSOR_MAP_DATA_TYPE_INT32, d.w, (unsigned long long)RQ * (d.N / 8), d.K / RQ, RQ * (d.N / 2ull), 32,
              W4T_ROWS / RQ, CU_TENSOR_MAP_SWIZZLE_128B) ||
         !map(&p.tx, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, d.x, d.K, d.M, d.ld_x * 2, 64, 8 * NT, CU_TENSOR_MAP_SWIZZLE_128B) ||
-        !map(&p.ts, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, d.s, d.N, (d.K + d.gs - 1) / d.gs, d.N * 2ull, W4D_FEATS, p.srows,
+        !map(&p.ts, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, d.s, d.N, (d.K + (long long)d.gs - 1) / d.gs, d.N * 2ull, W4D_FEATS, p.srows,
              CU_TENSOR_MAP_SWIZZLE_NONE))
         return FNX_EALIGN;
     static bool configured[FNX_MAX_DEVICES] = {};
-    static int resident[FNX_MAX_DEVICES][9] = {};            // clusters of each size the device holds at once
+    // clusters of each size the device holds at once, two CTAs to an SM whatever the ring's bytes
+    static int resident[FNX_MAX_DEVICES][9] = {};
     const int dev = current_device();
     if (!configured[dev]) {
         if (cudaFuncSetAttribute(w4_dense_tma_kernel<NT, SEG, QUAD>, cudaFuncAttributeMaxDynamicSharedMemorySize,

@@ -396,7 +396,7 @@ class DenseW4:
         if w4.dim() != 2 or w4.dtype != torch.int32 or sc.dim() != 2 or sc.dtype != BF16 or sc.device != w4.device:
             raise ValueError("DenseW4: int32 words [K, N/8] and bf16 scales [G, N] on one device expected")
         self.K, self.N, self.gs = w4.shape[0], w4.shape[1] * 8, gs
-        if self.K < 8 or self.K % 8 or self.N < 8 or gs < 16 or gs % 16 or tuple(sc.shape) != (-(-self.K // gs), self.N):
+        if self.K < 8 or self.K % 8 or self.N < 8 or not 16 <= gs < 2 ** 31 or gs % 16 or tuple(sc.shape) != (-(-self.K // gs), self.N):
             raise ValueError(f"DenseW4: K={self.K} must be a multiple of 8, gs={gs} of 16, and scales "
                              f"[{-(-self.K // max(gs, 1))}, {self.N}], not {tuple(sc.shape)}")
         _lib.require_cuda(w4)

@@ -35,7 +35,7 @@ def _rows(t, n, what, like):
 class GatedFFN:
     """``y = (silu(x Wg^T) * (x Wu^T)) Wd^T`` with ``w_gu`` bf16 ``[2I, H]`` (gate rows, then up rows)
     and ``w_down`` bf16 ``[O, I]``; H, I and O are multiples of 8.  The weights are read in place, so
-    an optimiser may update them between calls.
+    an optimiser may update them between a backward and the next forward.
 
     ``__call__(x)``: ``[.., H] -> [.., O]``.  ``forward_train(x)`` also returns what the backward
     needs (``x``, ``h`` and the pre-activations in fp32), ``backward(dy, saved)`` the gradients.
@@ -91,6 +91,8 @@ class GatedFFN:
         with the same ``saved``."""
         x2, h, gu, shape = saved
         M, dev = x2.shape[0], x2.device
+        if x2.shape[1] != self.H or h.shape[1] != self.I or dev != self.w_gu.device:
+            raise ValueError("GatedFFN.backward: saved comes from another block's forward_train")
         dy2, ld = _rows(dy, self.O, "gradient", self.w_gu)
         if dy2.shape[0] != M:
             raise ValueError(f"GatedFFN.backward: {dy2.shape[0]} rows for a forward of {M}")

@@ -9,7 +9,8 @@ def test_python_refusals():
     from fnx.engine import DenseW4
     w, s = torch.zeros(64, 4, dtype=torch.int32), torch.zeros(2, 32, dtype=BF16)
     for bad in ((w.float(), s, 32), (w[0], s, 32), (w, s.float(), 32), (w, s, 24), (w, s, 0), (w, s, 16), (w, s[:1], 32),
-                (w, s[:, :16], 32), (w[:60], s, 32), (w, s, -32)):
+                (w, s[:, :16], 32), (w[:60], s, 32), (w, s, -32),
+                (w, s[:1], 2 ** 32 + 128)):
         with pytest.raises(ValueError):
             DenseW4(*bad)
     with pytest.raises(RuntimeError):                       # no CPU path

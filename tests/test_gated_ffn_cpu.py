@@ -16,6 +16,19 @@ def test_python_refusals():
         GatedFFN(w, d)
 
 
+def test_backward_refuses_what_another_block_kept():
+    from fnx.gated_ffn import GatedFFN
+    blk = GatedFFN.__new__(GatedFFN)                        # (its own checks want a GPU)
+    blk.H, blk.I, blk.O, blk.w_gu = 16, 32, 24, torch.zeros(64, 16, dtype=BF16)
+    dy, x, h = (torch.zeros(4, n, dtype=BF16) for n in (24, 16, 32))
+    gu = torch.zeros(8, dtype=torch.uint8)
+    for x2, h2 in ((x[:, :8], h), (x, h[:, :24]), (x.to("meta"), h)):
+        with pytest.raises(ValueError, match="another block"):
+            blk.backward(dy, (x2, h2, gu, x2.shape))
+    with pytest.raises(ValueError, match="3 rows"):
+        blk.backward(dy[:3], (x, h, gu, x.shape))
+
+
 def test_abi_refusals():
     import build as fnx_build
     fnx_build.build()
