@@ -226,8 +226,8 @@ FNX_DEV float warp_sums32(float (&v)[32]) {
 // one the mean that the norm behind the block needs.
 // Bound: HBM would be (4 HC + 2) * H * 2 bytes a token (46 us for 4095 tokens of 4 x 2048); it takes 68 us,
 // with issue slots two thirds taken and the rest waiting at the token's two reductions.  Measured and not
-// kept: half as wide chunks with twice the threads (92 us), the gates' sums moved to the second reduction
-// (fewer instructions, a longer chain: 71 us).
+// kept (times with the forward, 120 us as it is): half as wide chunks with twice the threads (146), the gates'
+// sums moved to the second reduction (fewer instructions, a longer chain: 122).
 template <int HC>
 __global__ void __launch_bounds__(512, HC == 1 ? 2 : 1) inject_norm_bwd_kernel(const InjectNormBwdParams p) {
     extern __shared__ __align__(128) uint8_t stages[];

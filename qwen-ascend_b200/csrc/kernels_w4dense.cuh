@@ -10,7 +10,7 @@
 // Bound: the weight stream, K * N / 2 bytes read once, at long streams the issue of its conversion (8192 x
 // 28672, groups of 128, one token: 33.8 us, 3.6 TB/s of weights and scales; 4096 x 28672, groups of 32,
 // 16 tokens: 28.0 us), at short ones a launch and the cluster's sum (2048 x 5120, one token: 5.8 us).
-// The products run on mma.sync m16n8k16, which is far from its rate at this traffic (19 % busy): weights
+// The products run on mma.sync m16n8k16, which is far from its rate at this traffic (21 % busy): weights
 // are the 16-row operand straight from registers, the tokens the 8-column one.  A byte permute brings
 // the same byte of two rows' words into the two halves of a register, whose nibbles are then the (k, k+1)
 // pairs that the fragments want (nib_lo, nib_hi).
@@ -260,8 +260,8 @@ inline size_t w4_dense_smem(int M) {
 // the stream's depth nor a scale's latency is the warps' concern.  With the 128-byte swizzle the
 // fragment loads are free of bank conflicts for the natural order of k (lane t: rows 2t, 2t+1, 2t+8,
 // 2t+9 of a 16-row step).  A warp takes 64 features and half of the steps of a stage, and scales its
-// sums at the end of each group or stage.  Bound by issue: the exact conversion alone is 1.5
-// instructions a weight, 1.0 of them on the half-rate integer pipe.
+// sums at the end of each group or stage.  Bound by issue: the exact conversion alone is 1.25
+// instructions a weight, 0.75 of them on the half-rate integer pipe.
 constexpr int W4T_ROWS = 256;
 constexpr int W4T_MAX_STAGES = 3;
 constexpr int W4T_W_BYTES = W4T_ROWS * 128;

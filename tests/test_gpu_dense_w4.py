@@ -59,6 +59,13 @@ def test_wide(M, K, N, gs):
     check(lay, w, s, gs, torch.randn(M, K, generator=torch.Generator().manual_seed(M)).to(BF16).to(DEV))
 
 
+# fewer rows than a stage holds, by far, and as many columns as bring them to the ring
+@pytest.mark.parametrize("M,K,N,gs", [(2, 8, 2097160, 16), (9, 16, 1048608, 128), (1, 24, 699064, 32)])
+def test_few_rows_of_many_columns(M, K, N, gs):
+    lay, w, s = layer(K, N, gs)
+    check(lay, w, s, gs, torch.randn(M, K, generator=torch.Generator().manual_seed(M)).to(BF16).to(DEV))
+
+
 def test_activations_with_a_mean_and_outliers():
     """Values that are all positive, some a thousand times the others: nothing is taken from a large
     sum that the result does not hold itself."""

@@ -97,3 +97,43 @@ def test_decode_step_in_four_bits(b):
     want = st + (a * torch.sigmoid(a) * u) @ down.deq_w().double().t()
     near(out, want, 7)                                # state, normed, gate, up, act, down, itself
     near(nxt, rms64(want, w_after.double()), 7)
+
+
+FIRST_CALLS = """
+import sys
+sys.path.insert(0, sys.argv[1])
+import torch
+from fnx.engine import DenseW4
+from fnx.gated_ffn import GatedFFN
+from fnx.native_inject import inject_norm, inject_norm_backward
+r = lambda *s: (torch.randn(*s, device="cuda") * .1).bfloat16()
+ring = DenseW4(torch.randint(-2 ** 31, 2 ** 31, (4096, 512), device="cuda").int(), r(64, 4096), 64)
+short = DenseW4(torch.randint(-2 ** 31, 2 ** 31, (256, 32), device="cuda").int(), r(4, 256), 64)
+ffn, x, wide, wn = GatedFFN(r(512, 256), r(256, 256)), r(300, 256), r(3, 4096), r(256)
+
+def step():
+    state, normed = inject_norm(x, None, x, wn)
+    y, saved = ffn.forward_train(normed)
+    return (ring(wide), short(normed[:3]), state, y, *ffn.backward(y, saved),
+            *[t for t in inject_norm_backward(y, None, state, None, x, wn) if t is not None])
+
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = step()
+graph.replay()
+assert all(torch.equal(a, b) for a, b in zip(got, step()))
+print("same")
+"""
+
+
+def test_first_calls_of_a_process_inside_a_capture():
+    """What a first call sets up (shared-memory limits, occupancy) may be asked for while a stream captures."""
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    import fnx
+    out = subprocess.run([sys.executable, "-c", FIRST_CALLS, str(Path(fnx.__file__).parents[1])], capture_output=True,
+                         text=True, timeout=300)
+    assert out.returncode == 0 and out.stdout.strip() == "same", out.stderr[-2000:]
