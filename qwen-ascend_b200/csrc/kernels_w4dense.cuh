@@ -371,15 +371,18 @@ __global__ void __launch_bounds__(W4D_THREADS, 2) w4_dense_tma_kernel(const __gr
     const uint32_t x0 = W4T_W_BYTES + wk * (STEPS / 4) * NT * 1024 + g * 128 + (g << 4) + t * 4;
     const uint32_t c0 = W4T_W_BYTES + W4T_ROWS / 64 * NT * 1024 + word * 16;
 
+    bool alive = true;                                   // no wait has expired
     for (int j = 0, s = 0, ph = 0; j < ns; ++j) {
         // the slot of the stage before is refilled once its warps are done (the phase the other slots had)
         if (warp == 0 && j >= 1 && j - 1 + NS < ns) {
             const int sp = s ? s - 1 : NS - 1;
-            if (!__all_sync(0xffffffffu, mbar_wait(&empty[sp], s ? ph : ph ^ 1))) break;
+            alive = __all_sync(0xffffffffu, mbar_wait(&empty[sp], s ? ph : ph ^ 1));
+            if (!alive) break;
             if (elect_one()) fetch(j - 1 + NS, sp);
             __syncwarp();
         }
-        if (!__all_sync(0xffffffffu, mbar_wait(&full[s], ph))) break;
+        alive = __all_sync(0xffffffffu, mbar_wait(&full[s], ph));
+        if (!alive) break;
         const uint8_t* S = base + s * stage_bytes;
         const int first = (s0 + j) * (W4T_ROWS / 16), mine = first + wk * STEPS;
         int left = 0;                                    // steps to the end of the group
@@ -423,6 +426,8 @@ __global__ void __launch_bounds__(W4D_THREADS, 2) w4_dense_tma_kernel(const __gr
         if (lane == 0) mbar_arrive(&empty[s]);
         if (++s == NS) s = 0, ph ^= 1;
     }
+    if (!alive)                                          // time for the copies in flight to end
+        for (int i = 0; i < 200; ++i) __nanosleep(1000);
     __syncthreads();                                     // every stage is read: the sums reuse the ring
     w4_dense_finish<1, NT, TW * 8>(p, tot, reinterpret_cast<float*>(base), wn, wk, g, t, rank, CL, m0, mt);
 }
