@@ -512,9 +512,9 @@ __global__ void __launch_bounds__(512) inject_norm_bwd_wide_kernel(const InjectN
 
 // out[c] = bf16(sum over rows of part[row, c]) for c < n, rows in ascending order within each of the
 // block's eight row groups, whose sums are added in order (deterministic).  Column c < n0 goes to
-// out0, the rest to out1 (either may be NULL).
-__global__ void __launch_bounds__(256) column_sum_kernel(const float* __restrict__ part, bf16* __restrict__ out0,
-                                                         bf16* __restrict__ out1, int rows, int n0, int n) {
+// out0, the rest to out1 (either may be NULL).  The kernel before it still writes `part` while these
+// blocks start, so the pointers carry no __restrict__: its loads may not move above the wait.
+__global__ void __launch_bounds__(256) column_sum_kernel(const float* part, bf16* out0, bf16* out1, int rows, int n0, int n) {
     __shared__ float red[8][33];
     pdl_wait();
     pdl_launch_dependents();

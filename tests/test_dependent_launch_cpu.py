@@ -1,0 +1,37 @@
+"""What a kernel that starts before its predecessor on the stream has ended (a programmatic dependent
+launch) may and may not do, read off the sources: the memory it reads is still being written while it
+is resident, and only ``griddepcontrol.wait`` ends that."""
+import re
+from pathlib import Path
+
+CSRC = Path(__file__).resolve().parents[1] / "qwen-ascend_b200" / "csrc"
+
+
+def functions():
+    """``{name: (declaration, body)}`` of the kernels and device functions, comments left out."""
+    out = {}
+    for path in sorted(CSRC.glob("*.cuh")):
+        text = re.sub(r"//[^\n]*|/\*.*?\*/", "", path.read_text(), flags=re.S)
+        for m in re.finditer(r"^(?:__global__|FNX_DEV)\b[^;{}]*?\b(?!__launch)(\w+)\(([^;{}]*)\)\s*\{", text, flags=re.M):
+            depth, i = 1, m.end()
+            while depth:
+                depth += {"{": 1, "}": -1}.get(text[i], 0)
+                i += 1
+            out[m.group(1)] = (m.group(0), text[m.end():i])
+    return out
+
+
+FUNCTIONS = functions()
+DEPENDENT = {n for n, (d, b) in FUNCTIONS.items() if d.startswith("__global__") and "pdl_wait()" in b}
+
+
+def test_the_dependent_kernels_are_found():
+    assert {"column_sum_kernel", "decode_stream_kernel", "ffn_gemm_kernel", "ffn_small_kernel", "inject_norm_kernel",
+            "inject_norm_bwd_kernel", "inject_norm_bwd_wide_kernel", "w4_dense_kernel",
+            "w4_dense_tma_kernel"} <= DEPENDENT
+
+
+def test_no_dependent_kernel_declares_its_memory_unaliased():
+    """``__restrict__`` says that nobody else writes the memory while the kernel runs, which lets the
+    compiler load it early or through the read-only path: before the wait that makes it valid."""
+    assert [n for n in sorted(DEPENDENT) if "__restrict__" in FUNCTIONS[n][0]] == []
