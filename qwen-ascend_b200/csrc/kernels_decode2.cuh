@@ -582,15 +582,16 @@ FNX_DEV void d2_build_act(const tword* part, int MT, int ks, int I, bool shared_
 }
 
 // All M token rows into shared memory at entry (n16 16-byte words): four loads per thread in
-// flight before their stores.
-FNX_DEV void d2_stage_rows(const bf16* __restrict__ x, int n16, uint32_t* dst32) {
+// flight before their stores.  Ordinary loads: the kernel before this one may still write x while this
+// grid starts (programmatic dependent launch), which rules the read-only path out.
+FNX_DEV void d2_stage_rows(const bf16* x, int n16, uint32_t* dst32) {
     const uint4* src = reinterpret_cast<const uint4*>(x);
     uint4* dst = reinterpret_cast<uint4*>(dst32);
     for (int i0 = threadIdx.x; i0 < n16; i0 += 4 * D2_CTHREADS) {
         uint4 v[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u)
-            if (i0 + u * D2_CTHREADS < n16) v[u] = __ldg(src + i0 + u * D2_CTHREADS);
+            if (i0 + u * D2_CTHREADS < n16) v[u] = src[i0 + u * D2_CTHREADS];
 #pragma unroll
         for (int u = 0; u < 4; ++u)
             if (i0 + u * D2_CTHREADS < n16) dst[i0 + u * D2_CTHREADS] = v[u];
@@ -599,15 +600,15 @@ FNX_DEV void d2_stage_rows(const bf16* __restrict__ x, int n16, uint32_t* dst32)
 
 // A token row (H bf16, H % 256 == 0) into shared memory: 16-byte loads, up to two per thread in
 // flight before their stores (the loads may not pass a store through the generic pointer).
-FNX_DEV void d2_stage_row(const bf16* __restrict__ x, int H, uint32_t* xs2) {
+FNX_DEV void d2_stage_row(const bf16* x, int H, uint32_t* xs2) {
     const uint4* src = reinterpret_cast<const uint4*>(x);
     uint4* dst = reinterpret_cast<uint4*>(xs2);
     const int n = H / 8;
     for (int i = threadIdx.x; i < n; i += 2 * D2_CTHREADS) {
-        const uint4 a = __ldg(src + i);
+        const uint4 a = src[i];
         const bool two = i + D2_CTHREADS < n;
         uint4 b = a;
-        if (two) b = __ldg(src + i + D2_CTHREADS);
+        if (two) b = src[i + D2_CTHREADS];
         dst[i] = a;
         if (two) dst[i + D2_CTHREADS] = b;
     }

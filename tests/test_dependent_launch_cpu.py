@@ -35,3 +35,15 @@ def test_no_dependent_kernel_declares_its_memory_unaliased():
     """``__restrict__`` says that nobody else writes the memory while the kernel runs, which lets the
     compiler load it early or through the read-only path: before the wait that makes it valid."""
     assert [n for n in sorted(DEPENDENT) if "__restrict__" in FUNCTIONS[n][0]] == []
+
+
+def test_nothing_a_dependent_kernel_calls_reads_through_the_read_only_path():
+    """``__ldg`` carries the same promise to the compiler and the cache as ``__restrict__``."""
+    reached, todo = set(), sorted(DEPENDENT)
+    while todo:
+        name = todo.pop()
+        reached.add(name)
+        todo += [c for c in re.findall(r"\b(\w+)\s*(?:<[^;(){}]*>)?\(", FUNCTIONS[name][1])
+                 if c in FUNCTIONS and c not in reached]
+    assert "d2_stage_rows" in reached
+    assert [n for n in sorted(reached) if re.search(r"__ldg\b|\bld_nc_v4\b|ld\.global\.nc", FUNCTIONS[n][1])] == []
