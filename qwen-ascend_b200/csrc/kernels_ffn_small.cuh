@@ -153,6 +153,7 @@ __global__ void __launch_bounds__(FS_THREADS) ffn_small_kernel(const __grid_cons
         }
     } else if (warp == 1) {
         // ------------------------------------------------ MMA issue
+        pdl_wait();                                          // the bounded waits count from here
         auto multiply = [&](auto amn, auto bmn) {
             constexpr int AMN = decltype(amn)::value, BMN = decltype(bmn)::value;
             const uint32_t idesc = idesc_bf16_f32(128, BN) | ((uint32_t)AMN << 15) | ((uint32_t)BMN << 16);
@@ -180,6 +181,7 @@ __global__ void __launch_bounds__(FS_THREADS) ffn_small_kernel(const __grid_cons
         __syncwarp();
     } else if (warp < 6) {
         // ------------------------------------------------ this part's accumulators -> shared memory
+        pdl_wait();
         const bool ok = mbar_wait(&S.done, 0);
         if (!__all_sync(0xffffffffu, ok)) S.abort = 1;
         tc_fence_after();

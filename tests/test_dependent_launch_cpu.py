@@ -47,3 +47,17 @@ def test_nothing_a_dependent_kernel_calls_reads_through_the_read_only_path():
                  if c in FUNCTIONS and c not in reached]
     assert "d2_stage_rows" in reached
     assert [n for n in sorted(reached) if re.search(r"__ldg\b|\bld_nc_v4\b|ld\.global\.nc", FUNCTIONS[n][1])] == []
+
+
+def test_bounded_waits_begin_after_the_predecessor_has_ended():
+    """A bounded wait counts the time that a copy or a product may take.  Begun before the kernel's own
+    ``pdl_wait`` it would count what is left of the kernel before, and give up on a launch that lacks
+    nothing.  Every warp's path through a kernel therefore waits for the predecessor first."""
+    for name, roles in (("ffn_small_kernel", 3), ("ffn_gemm_kernel", 1), ("inject_norm_bwd_kernel", 1),
+                        ("w4_dense_tma_kernel", 1)):
+        # one pdl_wait at the head of the kernel, or (ffn_small) one in each warp's branch
+        branches = re.split(r"\} else if \(warp [=<]+ \d+\) \{", FUNCTIONS[name][1]) if roles > 1 else [FUNCTIONS[name][1]]
+        assert len(branches) == roles, name
+        for branch in branches:
+            first = re.search(r"\b(?:mbar_\w*wait\w*|mbar_spin|ffn_copy_tile\S*|ffn_multiply_tile\S*)\(", branch)
+            assert first and 0 <= branch.find("pdl_wait()") < first.start(), (name, branch[:60])
