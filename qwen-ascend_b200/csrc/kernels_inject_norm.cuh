@@ -277,10 +277,7 @@ __global__ void __launch_bounds__(512, HC == 1 ? 2 : 1) inject_norm_bwd_kernel(c
     int it = 0;
     for (long long t = blockIdx.x; t < p.batch; t += gridDim.x, ++it) {
         const int st = it & 1;
-        if (!mbar_wait(&full[st], (it >> 1) & 1)) {          // (every thread times out alike: the copy never came)
-            for (int i = 0; i < 200; ++i) __nanosleep(1000); // time for the copies in flight to end
-            break;
-        }
+        const bool landed = mbar_wait(&full[st], (it >> 1) & 1);
         const uint4* S = reinterpret_cast<const uint4*>(stages + (size_t)st * stage_bytes);
         const uint4 y4 = mine ? S[HC * nc + tid] : zero;
         // per branch s^2, e s, D z0, e z0, s z0 (five each), and y^2 last; z0 = y (1 + wp)
@@ -332,7 +329,11 @@ __global__ void __launch_bounds__(512, HC == 1 ? 2 : 1) inject_norm_bwd_kernel(c
             }
         }
         red[warp][lane] = warp_sums32(v);
-        __syncthreads();
+        // the block gives up as one (each thread's wait ends by its own clock)
+        if (!__syncthreads_and(landed)) {
+            for (int i = 0; i < 200; ++i) __nanosleep(1000); // time for the copies in flight to end
+            break;
+        }
         float tot = 0.f;                                     // value `lane`, over the block
         for (int i = 0; i < nw; ++i) tot += red[i][lane];
         // lane b: the scalars of branch b

@@ -61,3 +61,11 @@ def test_bounded_waits_begin_after_the_predecessor_has_ended():
         for branch in branches:
             first = re.search(r"\b(?:mbar_\w*wait\w*|mbar_spin|ffn_copy_tile\S*|ffn_multiply_tile\S*)\(", branch)
             assert first and 0 <= branch.find("pdl_wait()") < first.start(), (name, branch[:60])
+
+
+def test_a_block_gives_up_as_one():
+    """Each thread's own clock ends its bounded wait.  Where the threads meet at block barriers inside the
+    loop behind it, one that gave up alone would leave the others with sums that lack its part."""
+    body = FUNCTIONS["inject_norm_bwd_kernel"][1]
+    said = re.search(r"const bool (\w+) = mbar_wait\(&full", body)
+    assert said and f"if (!__syncthreads_and({said.group(1)}))" in body
