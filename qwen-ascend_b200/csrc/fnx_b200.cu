@@ -433,10 +433,12 @@ int inject_norm_launch(const InjectNormParams& p, int batch, cudaStream_t st) {
 size_t inject_norm_bwd_smem(int H, int HC) {
     return H <= 4096 ? (size_t)2 * (3 * HC + 1) * H * sizeof(bf16) : (size_t)(HC + 2) * H * sizeof(float);
 }
+// no more than fit at once: the blocks are persistent, and each writes its own partial sums
 int inject_norm_bwd_blocks(int batch, int H, int HC) {
     const int threads = H <= 4096 ? (H / 8 + 31) / 32 * 32 : 512;
+    const int regs = H <= 4096 && HC == 1 ? 64 : 128;                            // what their launch bounds allow
     int per_sm = (int)(220 * 1024 / (inject_norm_bwd_smem(H, HC) + 4096));       // shared memory
-    if (per_sm > 1024 / threads) per_sm = 1024 / threads;                        // registers
+    if (per_sm > 65536 / (regs * threads)) per_sm = 65536 / (regs * threads);    // registers
     if (per_sm > 4) per_sm = 4;
     if (per_sm < 1) per_sm = 1;
     const int g = per_sm * num_sms();
