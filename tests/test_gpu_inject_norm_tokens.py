@@ -46,3 +46,44 @@ def test_inputs_written_right_before_and_overwritten_right_after(T, H, HC):
         for x, w in zip(got, want[i % 2]):
             wrong += (x != w).sum()
     assert int(wrong) == 0
+
+
+def formulas(state, gate, values, w_next, w_post, d_state, d_normed, scale=0.75, eps=1e-6):
+    """The gradients in 64 bits from what the backward is handed: the stored state, not the unrounded one."""
+    T, H = values.shape[0], values.shape[-1]
+    HC = state.shape[-1] // H
+    s, y, wn, wp = state.double().view(T, HC, H), values.double().view(T, 1, H), w_next.double().view(HC, H), w_post.double()
+    D, e = d_state.double().view(T, HC, H), d_normed.double().view(T, HC, H)
+    g = scale * gate.double().view(T, HC, 1)
+    rs = ((s * s).mean(-1, keepdim=True) + eps) ** -0.5
+    rv = ((y * y).mean(-1, keepdim=True) + eps) ** -0.5
+    z = y * rv * (1 + wp)
+    d = D + rs * (e * (1 + wn) - s * rs ** 2 * (e * (1 + wn) * s).mean(-1, keepdim=True))
+    dz = (g * d).sum(1, keepdim=True)
+    dp = dz * (1 + wp)
+    dy = rv * (dp - y * rv ** 2 * (dp * y).mean(-1, keepdim=True))
+    return (d.reshape(state.shape), scale * (d * z).sum(-1).view(gate.shape), dy.reshape(values.shape),
+            (e * s * rs).sum(0).reshape(-1), (dz * y * rv).sum((0, 1)))
+
+
+@pytest.mark.parametrize("T,H,HC", MANY)
+def test_gradients_summed_over_many_tokens(T, H, HC):
+    """Against the formulas from the same stored state, so that only fp32 arithmetic and the last rounding
+    are between the two.  The rounding: 2^-8 of the value.  The arithmetic, relative to the largest value of
+    a gradient: a sum over T <= 6001 tokens has terms of at most sqrt(T) = 78 times its largest value in
+    sum (Cauchy, the largest of many columns being at least the root of its squared terms); it is made of
+    fewer than 41 tokens a block, 74 blocks a row group and 8 groups, 123 additions of 2^-24 each, and its
+    terms are good to 2^-20: 78 * (123 * 2^-24 + 2^-20) < 2^-10.  The others are good to 2^-20 of sums whose
+    terms exceed their largest value less than that.  One token left out of a sum, or counted twice, changes
+    it by a term of about 1 in 2^-10 of at most 400."""
+    hyper, gate, values, w_next, w_post, d_state, d_normed = a = inputs(T, H, HC, T)
+    got = step(*a)
+    want = formulas(got[0], gate, values, w_next, w_post, d_state, d_normed)
+    for name, x, w in zip(("d_hyper", "d_gate", "d_values", "d_w_next", "d_w_post"), got[2:], want):
+        assert x.dtype == BF16 and x.shape == w.shape
+        lim = 2 ** -8 * w.abs() + 2 ** -10 * w.abs().max()
+        err = (x.double() - w).abs()
+        assert bool((err <= lim).all()), (name, float((err / lim).max()))
+    again = step(*a)
+    for x, w in zip(again, got):
+        assert torch.equal(x, w)
