@@ -36,7 +36,22 @@ def inject(hyper, gate, values):
     return output
 
 
-def _inject_norm_args(hyper, gate, values, w_next, w_post):
+def _in_order(t, *dims):
+    """Whether ``t`` holds the values of an array ``dims`` in its order: axes merged, axes of length 1
+    added or the first axis split, but none exchanged."""
+    inner, at = 1, {1}
+    for d in dims[:0:-1]:
+        inner *= d
+        at.add(inner)
+    at.add(inner * dims[0])
+    n, cuts = 1, []
+    for d in t.shape[:0:-1]:
+        n *= d
+        cuts.append(n)
+    return all(c in at or (c % inner == 0 and (inner == 1 or inner in cuts)) for c in cuts)
+
+
+def _inject_norm_args(hyper, gate, values, w_next, w_post, grads=()):
     """Checks shared by the two directions -> ``(b, H, HC, whether a tensor has to be packed)``."""
     hs, vs = hyper.shape, values.shape
     b, W, H = hs[0], hs[-1], vs[-1]
@@ -56,6 +71,14 @@ def _inject_norm_args(hyper, gate, values, w_next, w_post):
     if not ok:
         raise ValueError(f"inject_norm: bf16 tensors on one device expected, a gate of {b * HC} values, w_next of {W}, "
                          f"w_post of {H}")
+    if (gate is not None and gate.shape[-1:] != (HC,) and not _in_order(gate, b, HC)
+            or w_next is not None and w_next.shape[-1:] != (W,) and not _in_order(w_next, HC, H)
+            or w_post is not None and w_post.shape[-1:] != (H,) and not _in_order(w_post, 1, H)):
+        raise ValueError(f"inject_norm: gate [{b}, 1, {HC}], w_next [{W}] and w_post [{H}] expected, axes in this order")
+    for t in grads:
+        if t is not None and (t.numel() != b * W or t.dtype is not BF16 or t.get_device() != at
+                              or t.shape[-1:] != (W,) and not _in_order(t, b, HC, H)):
+            raise ValueError("inject_norm_backward: gradients must be bf16, shaped and placed like state")
     if at < 0:
         _lib.require_cuda(hyper)
     return b, H, HC, pack
@@ -98,14 +121,11 @@ def inject_norm_backward(d_state, d_normed, state, gate, values, w_next=None, *,
     """Gradients of ``inject_norm`` from the gradients of its outputs (either may be ``None``: zero),
     the ``state`` it returned and its inputs: ``(d_hyper, d_gate, d_values, d_w_next, d_w_post)``,
     bf16 in the inputs' shapes, ``None`` where the input was ``None``.  Deterministic."""
-    b, H, HC, _ = _inject_norm_args(state, gate, values, w_next, w_post)
+    b, H, HC, _ = _inject_norm_args(state, gate, values, w_next, w_post, (d_state, d_normed))
     if d_state is None and d_normed is None:
         raise ValueError("inject_norm_backward: d_state or d_normed needed")
     if d_normed is not None and w_next is None:
         raise ValueError("inject_norm_backward: d_normed without w_next")
-    for t in (d_state, d_normed):
-        if t is not None and (t.numel() != state.numel() or t.dtype != torch.bfloat16 or t.device != state.device):
-            raise ValueError("inject_norm_backward: gradients must be bf16, shaped and placed like state")
     dev = state.device
     if _lib.elsewhere(state):
         with torch.cuda.device(dev):

@@ -22,3 +22,58 @@ def test_the_backward_launches_no_more_blocks_than_fit(H, HC):
     registers = 64 if HC == 1 and H <= 4096 else 128
     assert rest == 0 and blocks % sms == 0
     assert 1 <= blocks // sms <= max(1, 65536 // (registers * threads))
+
+
+def t(*shape):
+    return torch.zeros(shape, dtype=torch.bfloat16)
+
+
+HYPER, GATE, VALUES, W_NEXT, W_POST = t(8, 1, 4 * 64), t(8, 1, 4), t(8, 1, 64), t(256), t(64)
+
+
+@pytest.mark.parametrize("gate", [t(4, 8), t(1, 4, 8), t(4, 8, 1), t(2, 16)])
+def test_a_gate_in_another_order_is_refused(gate):
+    from fnx.native_inject import inject_norm, inject_norm_backward
+    with pytest.raises(ValueError):
+        inject_norm(HYPER, gate, VALUES, W_NEXT)
+    with pytest.raises(ValueError):
+        inject_norm_backward(HYPER, HYPER, HYPER, gate, VALUES, W_NEXT)
+
+
+@pytest.mark.parametrize("w_next,w_post", [(t(64, 4), None), (t(2, 128), None), (W_NEXT, t(8, 8)), (W_NEXT, t(2, 32))])
+def test_weights_in_another_order_are_refused(w_next, w_post):
+    from fnx.native_inject import inject_norm
+    with pytest.raises(ValueError):
+        inject_norm(HYPER, GATE, VALUES, w_next, w_post=w_post)
+
+
+@pytest.mark.parametrize("grad", [t(4, 8, 64), t(256, 8), t(256, 1, 8), t(8, 64, 4), t(4, 512)])
+def test_gradients_in_another_order_are_refused(grad):
+    from fnx.native_inject import inject_norm_backward
+    for pair in ((grad, None), (None, grad), (HYPER, grad)):
+        with pytest.raises(ValueError):
+            inject_norm_backward(*pair, HYPER, GATE, VALUES, W_NEXT)
+
+
+def test_every_row_major_form_of_the_same_values_is_taken():
+    """(as far as the check that there is a GPU, which comes last)"""
+    from fnx.native_inject import inject_norm, inject_norm_backward
+    for gate in (GATE, t(8, 4), t(8, 4, 1), t(32), t(2, 4, 4), None):
+        for w_next, w_post in ((W_NEXT, W_POST), (t(4, 64), t(1, 64)), (t(1, 256), t(64, 1)), (t(256, 1), None), (t(1, 256, 1), None)):
+            with pytest.raises(RuntimeError, match="CUDA"):
+                inject_norm(HYPER, gate, VALUES, w_next, w_post=w_post)
+    for grad in (HYPER, t(8, 256), t(8, 4, 64), t(32, 64), t(2, 4, 256), t(8 * 256)):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            inject_norm_backward(grad, grad, HYPER, GATE, VALUES, W_NEXT)
+    one, gate = t(8, 1, 64), t(8, 1, 1)                      # a single branch: any shape of b values
+    for g in (gate, t(8), t(2, 4), t(1, 8)):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            inject_norm(one, g, one, t(64))
+    first = t(1, 1, 256)                                     # a single token
+    for g in (t(4), t(1, 4), t(4, 1)):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            inject_norm(first, g, t(1, 64), W_NEXT)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        inject_norm(t(1, 1, 64), t(), t(1, 64), t(64))
+    with pytest.raises(RuntimeError, match="CUDA"):
+        inject_norm(t(0, 1, 256), t(0, 1, 4), t(0, 1, 64), W_NEXT)
