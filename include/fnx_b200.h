@@ -91,7 +91,7 @@ int fnx_inject_ex(void* h, void* y, void* g, void* out, int batch, int H, int HC
  * hyper, state, normed bf16 [batch, HC*H], gate bf16 [batch, HC] (NULL: 1), values bf16 [batch, H],
  * w_next bf16 [HC*H] (NULL with normed NULL: no second norm); rms(v) = sqrt(mean(v^2) + eps).
  * fp32 inside, each output rounded once (normed from the unrounded state).  state may be hyper.
- * H % 8 == 0, H <= 16384, HC <= 4, (HC + 2) * H <= 56000; all 16-byte aligned but gate. */
+ * H % 8 == 0, H <= 16384, HC <= 4, (HC + 2) * H <= 56000, eps >= 0; all 16-byte aligned but gate. */
 int fnx_inject_norm(const void* hyper, const void* gate, const void* values, const void* w_post, const void* w_next,
                     void* state, void* normed, int batch, int H, int HC, float scale, float eps, void* stream);
 /* Its gradients, from its stored state and its inputs: d_state, d_normed bf16 [batch, HC*H] (one of

@@ -464,6 +464,7 @@ FNX_API int fnx_inject_norm(const void* hyper, const void* gate, const void* val
                             const void* w_next, void* state, void* normed, int batch, int H, int HC, float scale,
                             float eps, void* stream) {
     if (!inject_norm_shape(batch, H, HC)) return FNX_ESHAPE;
+    if (!(eps >= 0.f)) return FNX_EARG;
     if (batch == 0) return FNX_OK;                    // an empty tensor has no address
     if (!hyper || !values || !state || (!w_next != !normed)) return FNX_EARG;
     if (!aligned16(hyper) || !aligned16(values) || !aligned16(state) || (w_post && !aligned16(w_post)) ||
@@ -487,6 +488,7 @@ FNX_API int fnx_inject_norm_backward(const void* d_state, const void* d_normed, 
                                      void* d_gate, void* d_values, void* d_w_post, void* d_w_next, int batch, int H,
                                      int HC, float scale, float eps, void* ws, size_t ws_bytes, void* stream) {
     if (!inject_norm_shape(batch, H, HC)) return FNX_ESHAPE;
+    if (!(eps >= 0.f)) return FNX_EARG;
     if (batch && ((!d_state && !d_normed) || !state || !values || !d_hyper || !d_values || (d_gate && !gate)))
         return FNX_EARG;                              // an empty tensor has no address
     if ((d_normed && !w_next) || (d_w_post && !w_post) || (d_w_next && !w_next)) return FNX_EARG;

@@ -51,7 +51,7 @@ def _in_order(t, *dims):
     return all(c in at or (c % inner == 0 and (inner == 1 or inner in cuts)) for c in cuts)
 
 
-def _inject_norm_args(hyper, gate, values, w_next, w_post, grads=()):
+def _inject_norm_args(hyper, gate, values, w_next, w_post, eps, grads=()):
     """Checks shared by the two directions -> ``(b, H, HC, whether a tensor has to be packed)``."""
     hs, vs = hyper.shape, values.shape
     b, W, H = hs[0], hs[-1], vs[-1]
@@ -61,6 +61,8 @@ def _inject_norm_args(hyper, gate, values, w_next, w_post, grads=()):
     if H % 8 or H > 16384 or HC > 4 or (HC + 2) * H > 56000:
         raise ValueError(f"inject_norm: H={H}, HC={HC}: H must be a multiple of 8 up to 16384, HC at most 4 and "
                          "(HC + 2) * H at most 56000")
+    if not eps >= 0:
+        raise ValueError(f"inject_norm: eps={eps} must not be negative")
     at = hyper.get_device()
     pack = not (hyper.is_contiguous() and values.is_contiguous())
     ok = hyper.dtype is BF16 and values.dtype is BF16 and values.get_device() == at
@@ -99,7 +101,7 @@ def inject_norm(hyper, gate, values, w_next=None, *, w_post=None, scale=1.0, eps
     ``w_next`` ``[HC*H]``, ``w_post`` ``[H]``; HC = 1 is an ordinary residual stream.  Returns
     ``(state, normed)`` shaped like ``hyper``.  fp32 inside, each output rounded once; ``normed``
     comes from the unrounded state, so it can differ by one rounding from a norm of ``state``."""
-    b, H, HC, pack = _inject_norm_args(hyper, gate, values, w_next, w_post)
+    b, H, HC, pack = _inject_norm_args(hyper, gate, values, w_next, w_post, eps)
     dev = hyper.device
     if _lib.elsewhere(hyper):
         with torch.cuda.device(dev):
@@ -121,7 +123,7 @@ def inject_norm_backward(d_state, d_normed, state, gate, values, w_next=None, *,
     """Gradients of ``inject_norm`` from the gradients of its outputs (either may be ``None``: zero),
     the ``state`` it returned and its inputs: ``(d_hyper, d_gate, d_values, d_w_next, d_w_post)``,
     bf16 in the inputs' shapes, ``None`` where the input was ``None``.  Deterministic."""
-    b, H, HC, _ = _inject_norm_args(state, gate, values, w_next, w_post, (d_state, d_normed))
+    b, H, HC, _ = _inject_norm_args(state, gate, values, w_next, w_post, eps, (d_state, d_normed))
     if d_state is None and d_normed is None:
         raise ValueError("inject_norm_backward: d_state or d_normed needed")
     if d_normed is not None and w_next is None:

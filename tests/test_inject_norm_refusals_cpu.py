@@ -77,3 +77,15 @@ def test_every_row_major_form_of_the_same_values_is_taken():
         inject_norm(t(1, 1, 64), t(), t(1, 64), t(64))
     with pytest.raises(RuntimeError, match="CUDA"):
         inject_norm(t(0, 1, 256), t(0, 1, 4), t(0, 1, 64), W_NEXT)
+
+
+@pytest.mark.parametrize("eps", [-1e-6, float("nan")])
+def test_an_eps_that_is_no_bound_is_refused(eps):
+    from fnx.native_inject import inject_norm, inject_norm_backward
+    with pytest.raises(ValueError, match="eps"):
+        inject_norm(HYPER, GATE, VALUES, W_NEXT, eps=eps)
+    with pytest.raises(ValueError, match="eps"):
+        inject_norm_backward(HYPER, HYPER, HYPER, GATE, VALUES, W_NEXT, eps=eps)
+    L = lib()
+    assert L.fnx_inject_norm(16, 16, 16, None, None, 16, None, 0, 64, 4, 1.0, eps, None) == -1
+    assert L.fnx_inject_norm_backward(*[16] * 12, 0, 64, 4, 1.0, eps, 16, 0, None) == -1
