@@ -138,6 +138,15 @@ def ptr(t) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+def no_autograd(what: str, *tensors):
+    """Refuses tensors that carry an autograd graph into a plain function, which would cut it silently."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{what}: an input requires a gradient, which this call does not record; detach it or "
+                                 "call under torch.no_grad()")
+
+
 def check(rc: int, what: str):
     if rc:
         raise RuntimeError(f"{what} launch rejected: {rc}")

@@ -390,7 +390,8 @@ class DenseW4:
     ``x [.., K] @ (q * s) -> bf16 [.., N]`` on the weight-streaming GEMV, accumulated in fp32 with the
     scale applied to each group's exact sum (no weight is rounded, unlike the expert GEMM's
     ``bf16(q * s)``).  The weights are read once for up to 16 rows; more rows are right but read
-    them again every 16.  K and N are multiples of 8, ``gs`` of 16."""
+    them again every 16.  K and N are multiples of 8, ``gs`` of 16.  There is no gradient: an ``x``
+    that requires one while gradients are recorded is refused."""
 
     def __init__(self, w4, sc, gs):
         if w4.dim() != 2 or w4.dtype != torch.int32 or sc.dim() != 2 or sc.dtype != BF16 or sc.device != w4.device:
@@ -407,6 +408,7 @@ class DenseW4:
 
     def __call__(self, x):
         shape, dev, K = x.shape, self.w4.device, self.K
+        _lib.no_autograd("DenseW4", x)
         if shape[-1] != K or x.device != dev:
             raise ValueError(f"DenseW4: rows of {K} on {dev} expected, got {tuple(shape)} on {x.device}")
         if _lib.elsewhere(x):

@@ -39,7 +39,8 @@ class GatedFFN:
 
     ``__call__(x)``: ``[.., H] -> [.., O]``.  ``forward_train(x)`` also returns what the backward
     needs (``x``, ``h`` and the pre-activations in fp32), ``backward(dy, saved)`` the gradients.
-    ``gated(x)`` is the first half alone, ``h [.., I]``."""
+    ``gated(x)`` is the first half alone, ``h [.., I]``.  No call is an autograd node: ``__call__`` and
+    ``gated`` refuse an ``x`` that requires a gradient while gradients are recorded."""
 
     def __init__(self, w_gu, w_down):
         if (w_gu.dim() != 2 or w_down.dim() != 2 or w_gu.dtype != BF16 or w_down.dtype != BF16
@@ -72,11 +73,13 @@ class GatedFFN:
         return x2, h, gu, y
 
     def __call__(self, x):
+        _lib.no_autograd("GatedFFN", x)
         y = self._forward(x, False, True)[3]
         return y if x.dim() == 2 else y.view(*x.shape[:-1], self.O)
 
     def gated(self, x):
         """``h = silu(x Wg^T) * (x Wu^T)``: ``[.., H] -> [.., I]``."""
+        _lib.no_autograd("GatedFFN.gated", x)
         h = self._forward(x, False, False)[1]
         return h if x.dim() == 2 else h.view(*x.shape[:-1], self.I)
 

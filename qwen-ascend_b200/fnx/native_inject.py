@@ -100,7 +100,10 @@ def inject_norm(hyper, gate, values, w_next=None, *, w_post=None, scale=1.0, eps
     ``[b, 1, HC*H]``, ``gate`` bf16 ``[b, 1, HC]`` or ``None`` (1), ``values`` bf16 ``[b, 1, H]``,
     ``w_next`` ``[HC*H]``, ``w_post`` ``[H]``; HC = 1 is an ordinary residual stream.  Returns
     ``(state, normed)`` shaped like ``hyper``.  fp32 inside, each output rounded once; ``normed``
-    comes from the unrounded state, so it can differ by one rounding from a norm of ``state``."""
+    comes from the unrounded state, so it can differ by one rounding from a norm of ``state``.  Not an
+    autograd node: a ``hyper``, ``gate`` or ``values`` that requires a gradient while gradients are
+    recorded is refused; ``inject_norm_backward`` gives the gradients."""
+    _lib.no_autograd("inject_norm", hyper, gate, values)
     b, H, HC, pack = _inject_norm_args(hyper, gate, values, w_next, w_post, eps)
     dev = hyper.device
     if _lib.elsewhere(hyper):
