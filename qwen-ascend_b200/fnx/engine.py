@@ -408,7 +408,8 @@ class DenseW4:
 
     def __call__(self, x):
         shape, dev, K = x.shape, self.w4.device, self.K
-        _lib.no_autograd("DenseW4", x)
+        if x.requires_grad:
+            _lib.no_autograd("DenseW4", x)
         if shape[-1] != K or x.device != dev:
             raise ValueError(f"DenseW4: rows of {K} on {dev} expected, got {tuple(shape)} on {x.device}")
         if _lib.elsewhere(x):

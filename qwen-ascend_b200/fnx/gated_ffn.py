@@ -73,7 +73,8 @@ class GatedFFN:
         return x2, h, gu, y
 
     def __call__(self, x):
-        _lib.no_autograd("GatedFFN", x)
+        if x.requires_grad:
+            _lib.no_autograd("GatedFFN", x)
         y = self._forward(x, False, True)[3]
         return y if x.dim() == 2 else y.view(*x.shape[:-1], self.O)
 

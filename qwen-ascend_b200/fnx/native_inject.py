@@ -66,20 +66,17 @@ def _inject_norm_args(hyper, gate, values, w_next, w_post, eps, grads=()):
     at = hyper.get_device()
     pack = not (hyper.is_contiguous() and values.is_contiguous())
     ok = hyper.dtype is BF16 and values.dtype is BF16 and values.get_device() == at
-    for t, n in ((gate, b * HC), (w_next, W), (w_post, H)):
+    for t, n, rows in ((gate, b * HC, b), (w_next, W, HC), (w_post, H, 1)):
         if t is not None:
-            ok = ok and t.dtype is BF16 and t.get_device() == at and t.numel() == n
+            ok = ok and t.dtype is BF16 and t.get_device() == at and t.numel() == n and (
+                t.dim() < 2 or t.size(-1) * rows == n or _in_order(t, rows, n // max(rows, 1)))
             pack = pack or not t.is_contiguous()
     if not ok:
-        raise ValueError(f"inject_norm: bf16 tensors on one device expected, a gate of {b * HC} values, w_next of {W}, "
-                         f"w_post of {H}")
-    if (gate is not None and gate.shape[-1:] != (HC,) and not _in_order(gate, b, HC)
-            or w_next is not None and w_next.shape[-1:] != (W,) and not _in_order(w_next, HC, H)
-            or w_post is not None and w_post.shape[-1:] != (H,) and not _in_order(w_post, 1, H)):
-        raise ValueError(f"inject_norm: gate [{b}, 1, {HC}], w_next [{W}] and w_post [{H}] expected, axes in this order")
+        raise ValueError(f"inject_norm: bf16 tensors on one device expected, a gate [{b}, 1, {HC}], w_next [{W}], "
+                         f"w_post [{H}], axes in this order")
     for t in grads:
         if t is not None and (t.numel() != b * W or t.dtype is not BF16 or t.get_device() != at
-                              or t.shape[-1:] != (W,) and not _in_order(t, b, HC, H)):
+                              or t.dim() > 1 and t.size(-1) != W and not _in_order(t, b, HC, H)):
             raise ValueError("inject_norm_backward: gradients must be bf16, shaped and placed like state")
     if at < 0:
         _lib.require_cuda(hyper)
@@ -103,7 +100,8 @@ def inject_norm(hyper, gate, values, w_next=None, *, w_post=None, scale=1.0, eps
     comes from the unrounded state, so it can differ by one rounding from a norm of ``state``.  Not an
     autograd node: a ``hyper``, ``gate`` or ``values`` that requires a gradient while gradients are
     recorded is refused; ``inject_norm_backward`` gives the gradients."""
-    _lib.no_autograd("inject_norm", hyper, gate, values)
+    if hyper.requires_grad or values.requires_grad or (gate is not None and gate.requires_grad):
+        _lib.no_autograd("inject_norm", hyper, gate, values)
     b, H, HC, pack = _inject_norm_args(hyper, gate, values, w_next, w_post, eps)
     dev = hyper.device
     if _lib.elsewhere(hyper):
