@@ -52,7 +52,8 @@ def _in_order(t, *dims):
 
 
 def _inject_norm_args(hyper, gate, values, w_next, w_post, eps, grads=()):
-    """Checks shared by the two directions -> ``(b, H, HC, whether a tensor has to be packed)``."""
+    """Checks shared by the two directions -> ``(b, H, HC, whether a tensor has to be packed,
+    device index)``."""
     hs, vs = hyper.shape, values.shape
     b, W, H = hs[0], hs[-1], vs[-1]
     if H < 1 or W % H or values.numel() != b * H or hyper.numel() != b * W:
@@ -69,18 +70,18 @@ def _inject_norm_args(hyper, gate, values, w_next, w_post, eps, grads=()):
     for t, n, rows in ((gate, b * HC, b), (w_next, W, HC), (w_post, H, 1)):
         if t is not None:
             ok = ok and t.dtype is BF16 and t.get_device() == at and t.numel() == n and (
-                t.dim() < 2 or t.size(-1) * rows == n or _in_order(t, rows, n // max(rows, 1)))
+                t.dim() < 2 or t.shape[-1] * rows == n or _in_order(t, rows, n // max(rows, 1)))
             pack = pack or not t.is_contiguous()
     if not ok:
         raise ValueError(f"inject_norm: bf16 tensors on one device expected, a gate [{b}, 1, {HC}], w_next [{W}], "
                          f"w_post [{H}], axes in this order")
     for t in grads:
         if t is not None and (t.numel() != b * W or t.dtype is not BF16 or t.get_device() != at
-                              or t.dim() > 1 and t.size(-1) != W and not _in_order(t, b, HC, H)):
+                              or t.dim() > 1 and t.shape[-1] != W and not _in_order(t, b, HC, H)):
             raise ValueError("inject_norm_backward: gradients must be bf16, shaped and placed like state")
     if at < 0:
         _lib.require_cuda(hyper)
-    return b, H, HC, pack
+    return b, H, HC, pack, at
 
 
 def _packed(*ts):
@@ -102,10 +103,9 @@ def inject_norm(hyper, gate, values, w_next=None, *, w_post=None, scale=1.0, eps
     recorded is refused; ``inject_norm_backward`` gives the gradients."""
     if hyper.requires_grad or values.requires_grad or (gate is not None and gate.requires_grad):
         _lib.no_autograd("inject_norm", hyper, gate, values)
-    b, H, HC, pack = _inject_norm_args(hyper, gate, values, w_next, w_post, eps)
-    dev = hyper.device
-    if _lib.elsewhere(hyper):
-        with torch.cuda.device(dev):
+    b, H, HC, pack, at = _inject_norm_args(hyper, gate, values, w_next, w_post, eps)
+    if at != torch._C._cuda_getDevice():              # (see _lib.elsewhere)
+        with torch.cuda.device(at):
             return inject_norm(hyper, gate, values, w_next, w_post=w_post, scale=scale, eps=eps)
     if pack:
         hyper, gate, values, w_next, w_post = _packed(hyper, gate, values, w_next, w_post)
@@ -113,7 +113,8 @@ def inject_norm(hyper, gate, values, w_next=None, *, w_post=None, scale=1.0, eps
     normed = None if w_next is None else torch.empty_like(hyper)
     ptr = _lib.ptr
     rc = _lib.lib().fnx_inject_norm(hyper.data_ptr(), ptr(gate), values.data_ptr(), ptr(w_post), ptr(w_next),
-                                    state.data_ptr(), ptr(normed), b, H, HC, scale, eps, _lib.raw_stream(dev))
+                                    state.data_ptr(), ptr(normed), b, H, HC, scale, eps,
+                                    torch._C._cuda_getCurrentRawStream(at))
     if rc == _lib.EALIGN and not pack:                # a view that starts off a 16-byte boundary
         return inject_norm(*_packed(hyper, gate, values, w_next), w_post=_packed(w_post)[0], scale=scale, eps=eps)
     _lib.check(rc, "residual injection with norms")
@@ -124,7 +125,7 @@ def inject_norm_backward(d_state, d_normed, state, gate, values, w_next=None, *,
     """Gradients of ``inject_norm`` from the gradients of its outputs (either may be ``None``: zero),
     the ``state`` it returned and its inputs: ``(d_hyper, d_gate, d_values, d_w_next, d_w_post)``,
     bf16 in the inputs' shapes, ``None`` where the input was ``None``.  Deterministic."""
-    b, H, HC, _ = _inject_norm_args(state, gate, values, w_next, w_post, eps, (d_state, d_normed))
+    b, H, HC, _, _ = _inject_norm_args(state, gate, values, w_next, w_post, eps, (d_state, d_normed))
     if d_state is None and d_normed is None:
         raise ValueError("inject_norm_backward: d_state or d_normed needed")
     if d_normed is not None and w_next is None:
