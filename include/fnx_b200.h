@@ -301,7 +301,8 @@ int fnx_w8a16_gemm_ws(const void* x, const void* w8t, const void* sc, void* y, i
  * int32 [K, N/8] int4pack (tools/repack_w4a16.py:64-70, one expert), scales bf16 [ceil(K/gs), N] (the
  * last group may be short), x bf16 [M, ld_x].  fp32 accumulation, weights not rounded, deterministic.
  * K % 8 == 0, N % 8 == 0, gs % 16 == 0, ld_x % 4 == 0; pointers 16-byte aligned.  M <= 1048560; the
- * weights are read once for up to 16 rows. */
+ * weights are read once for up to 16 rows.  Long weight streams are fastest with ld_x % 8 == 0 (tensor
+ * copies; other strides take the direct loads whatever the size). */
 int fnx_w4a16_gemv(const void* x, long long ld_x, const void* w4, const void* scales, void* y, int M, int K, int N,
                    int gs, void* stream);
 

@@ -1348,8 +1348,8 @@ int ffn_products(const FfnGemm* g, int count, float* gu, bool chained, bool foll
         else if (g[i].M > box_rows) box_rows = g[i].M;
     }
     // Few rows: the weights' bytes are the work, 128-row tiles of them (64 where even eight parts of K
-    // leave SMs free).  More rows: 64 columns, while the tiles fit the SMs twice; beyond that CTA pairs,
-    // unless their 256 rows would be half empty.
+    // leave SMs free).  More rows: 64 columns for up to 256 tiles (of the 296 that 148 SMs hold at two
+    // each); beyond that CTA pairs, unless their 256 rows would be half empty.
     const bool few = rows <= 64, fits = t64 <= 256;
     if (!few && !fits && rows > 128) return ffn_pair_launch<EPI>(g, count, gu, followed, st);
     const int BN = few ? (t64 * FS_MAX_CL <= num_sms() ? 64 : 128) : fits ? 64 : 128;
@@ -1419,7 +1419,11 @@ FNX_API int fnx_gated_ffn_backward(const void* dy, long long ld_dy, const void* 
     const FfnGemm dh{dy, w_down, dgu, (bf16*)dgu + I, ld_dy, I, 2LL * I, M, I, O, 0, 1};
     rc = ffn_products<FF_DGATE>(&dh, 1, (float*)const_cast<void*>(saved), false, dx || dw_gu || dw_down, st);
     if (rc) return rc;
-    // the three products that follow, in one launch, the one with the longest tiles first
+    // The three products that follow, in one launch.  dx comes first: a tile of it sums over 2I, one of the
+    // weight gradients over M, and the longest tiles should start first.  With M > 2I that order is the wrong
+    // one, and the last tiles of the weight gradients end the launch late (counted in k-blocks of the busiest
+    // CTA pair against an even share: 168 / 112 at 4096 x 2560 x 640, 64 / 9 at 4096 x 512 x 256; with the
+    // forward these take 125 and 46 us).
     FfnGemm g[FF_MAX_PRODUCTS];
     int n = 0;
     if (dx) g[n++] = FfnGemm{dgu, w_gu, dx, nullptr, 2LL * I, H, H, M, H, 2 * I, 0, 1};
@@ -1576,7 +1580,8 @@ FNX_API int fnx_w4a16_gemv(const void* x, long long ld_x, const void* w4, const 
     // From 8 MB of weights on the ring of TMA copies (2048 x 16384, 8 tokens: 8.1 us against 15.6; 6352 x
     // 13768, whose rows are off 16 bytes: 17.6 against 27.5).  Below, the direct loads: the ring takes
     // about 1 us less on the GPU (2048 x 5120: 4.9 against 5.8) but a call from Python half a microsecond
-    // more (4096 x 2560: 8.8 against 8.2), and that is what such a short call waits for.
+    // more (4096 x 2560: 8.8 against 8.2, of which its three tensor maps are a fifth), and that is what such a
+    // short eager call waits for.  A captured one pays the microsecond.
     if (ld_x % 8 == 0 && (long long)K * N >= 16 << 20)
         return NT == 2 ? w4_dense_tma_launch<2>(p, st) : w4_dense_tma_launch<1>(p, st);
     // parts of K until the CTAs fill the SMs twice, at least 16 steps of 16 rows each

@@ -142,8 +142,10 @@ FNX_DEV bool mbar_spin(uint64_t* bar, uint32_t parity) {
     }
 }
 
-// sigmoid(g) for the activation: exponential and reciprocal are the fast forms (2^-21 relative), whose
-// error is far below the bf16 rounding of every result
+// sigmoid(g) for the activation: exponential and reciprocal are the fast forms.  The exponential's error
+// grows with |g| (2 + 1.173 |g| units of its last place), so towards negative g, where the sigmoid is that
+// exponential's inverse, the result is good to 2^-21 at g = -2, 2^-18 at -20 and 2^-16 at -87: far below
+// the bf16 rounding of every result.  Below -87.3 the sigmoid is 0 (it is smaller than 2^-126).
 FNX_DEV float fast_sigmoid(float g) { return __fdividef(1.0f, 1.0f + __expf(-g)); }
 
 // Tile t of the launch: its product, and within it groups of 8 row tiles, columns outside, rows

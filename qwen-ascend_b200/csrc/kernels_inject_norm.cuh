@@ -225,7 +225,8 @@ FNX_DEV float warp_sums32(float (&v)[32]) {
 // two stages while the token before is computed.  One reduction gives all sums over the rows, a second
 // one the mean that the norm behind the block needs.
 // Bound: HBM would be (4 HC + 2) * H * 2 bytes a token (46 us for 4095 tokens of 4 x 2048); it takes 68 us,
-// with issue slots two thirds taken and the rest waiting at the token's two reductions.  Measured and not
+// with issue slots two thirds taken and the rest waiting at the token's two reductions (2 x 2048: 47 us with
+// the column sums, 26 of them bytes).  Measured and not
 // kept (times with the forward, 120 us as it is): half as wide chunks with twice the threads (146), the gates'
 // sums moved to the second reduction (fewer instructions, a longer chain: 122).
 template <int HC>
@@ -413,7 +414,10 @@ __global__ void __launch_bounds__(512, HC == 1 ? 2 : 1) inject_norm_bwd_kernel(c
 }
 
 // The backward for wider rows: every thread owns several chunks, whose weight-gradient sums it keeps in
-// shared memory over all of its block's tokens, and reads the rows twice.
+// shared memory over all of its block's tokens, and reads the rows twice, with one block on an SM (its 512
+// threads take the registers).  Bound: the latency of those reads and of a block reduction for every branch
+// and token, with nothing in flight under them: 4096 tokens of 2 x 4104 take 463 us with the forward, where the
+// bytes would be 72.
 __global__ void __launch_bounds__(512) inject_norm_bwd_wide_kernel(const InjectNormBwdParams p) {
     extern __shared__ __align__(16) float acc[];           // [(HC + 1) * H], then dz [H]
     __shared__ float red[32 * 6];
